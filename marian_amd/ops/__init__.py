@@ -238,6 +238,93 @@ def layer_norm_residual(x: torch.Tensor, res: torch.Tensor,
 
 
 # ---------------------------------------------------------------------------
+# Gated linear recurrence (ref: rnn/cells.h SSRU)
+# ---------------------------------------------------------------------------
+
+def gated_scan(x: torch.Tensor, gate: torch.Tensor,
+               state: Optional[torch.Tensor] = None,
+               lens: Optional[torch.Tensor] = None, reverse: bool = False,
+               act: str = "none"):
+    """Gated linear recurrence over sequences; returns (y, last).
+
+        f_t = sigmoid(gate_t);  c_t = f_t c_{t-1} + (1 - f_t) x_t
+        y_t = act(c_t)          act: "none" | "relu"
+
+    x, gate: [B, T, D], fp32 / bf16 / fp16, any batch and time strides (the
+    last dimension is copied if it is not dense). state: float32 [B, D], the
+    state before the first step (default zeros). lens: int32 [B]; the steps
+    of row b are its first lens[b] positions (clamped to 0..T); what lies
+    behind them is ignored, y is 0 there and so are its gradients.
+    reverse: the steps run from position lens[b]-1 down to 0.
+    y: [B, T, D] in x's dtype; last: float32 [B, D], the state after the last
+    step (`state` itself for a row of no steps). States are held in 32 bits.
+    Differentiable once in x, gate and state.
+    """
+    from ._gated_scan import (GatedScanFn, check_scan, dense_rows,
+                              gated_scan_torch)
+    check_scan("gated_scan", x, gate, state, lens, act, 3)
+    if _on_gpu(x):
+        return GatedScanFn.apply(
+            dense_rows(x), dense_rows(gate),
+            None if state is None else state.contiguous(),
+            None if lens is None else lens.contiguous(), bool(reverse), act)
+    return gated_scan_torch(x, gate, state, lens, reverse, act)
+
+
+def gated_scan_xg(xg: torch.Tensor, state: Optional[torch.Tensor] = None,
+                  lens: Optional[torch.Tensor] = None, reverse: bool = False,
+                  act: str = "none"):
+    """gated_scan on a fused projection xg [B, T, 2D], values first, gates
+    second: read in place, and one gradient buffer comes out."""
+    from ._gated_scan import (GatedScanXGFn, check_scan, dense_rows,
+                              gated_scan_torch)
+    if xg.dim() != 3 or xg.shape[-1] % 2:
+        raise ValueError("gated_scan_xg: xg must be [B, T, 2D], got "
+                         f"{tuple(xg.shape)}")
+    d = xg.shape[-1] // 2
+    check_scan("gated_scan_xg", xg[..., :d], xg[..., d:], state, lens, act, 3)
+    if _on_gpu(xg):
+        return GatedScanXGFn.apply(
+            dense_rows(xg), None if state is None else state.contiguous(),
+            None if lens is None else lens.contiguous(), bool(reverse), act)
+    return gated_scan_torch(xg[..., :d], xg[..., d:], state, lens, reverse,
+                            act)
+
+
+def gated_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor,
+               act: str = "none", inplace: bool = False):
+    """One step of gated_scan for each row; returns (y, new_state).
+
+    x, gate: [N, D] (rows may be strided); state: float32 [N, D]. inplace
+    writes the new state over `state` (which must be dense) and returns it,
+    as a captured decode step needs; that call has no gradient. Otherwise a
+    call that needs gradients runs as gated_scan over one position.
+    """
+    from ._gated_scan import check_scan, dense_rows, gated_scan_torch
+    if state is None:
+        raise ValueError("gated_step: state is required")
+    check_scan("gated_step", x, gate, state, None, act, 2)
+    grad = torch.is_grad_enabled() and (
+        x.requires_grad or gate.requires_grad or state.requires_grad)
+    if inplace:
+        if grad:
+            raise ValueError("gated_step: inplace has no gradient")
+        if not state.is_contiguous():
+            raise ValueError("gated_step: inplace needs a dense state")
+    elif grad:
+        y, new = gated_scan(x[:, None], gate[:, None], state, act=act)
+        return y[:, 0], new
+    if _on_gpu(x):
+        state = state.contiguous()
+        out = state if inplace else torch.empty_like(state)
+        y = hip_ext(required=True).gated_step(dense_rows(x), dense_rows(gate),
+                                              state, out, act)
+        return y, out
+    y, new = gated_scan_torch(x[:, None], gate[:, None], state, act=act)
+    return y[:, 0], state.copy_(new) if inplace else new
+
+
+# ---------------------------------------------------------------------------
 # Attention  (ref: composite ProdBatched+mask+gSoftmax+ProdBatched;
 #             rebuilt as a fused flash-style CDNA4 kernel)
 # ---------------------------------------------------------------------------

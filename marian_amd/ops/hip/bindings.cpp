@@ -56,6 +56,23 @@ std::vector<torch::Tensor> attention_bwd(torch::Tensor q, torch::Tensor k,
                                          c10::optional<torch::Tensor> kv_lens,
                                          bool causal, double scale);
 
+std::vector<torch::Tensor> gated_scan_fwd(torch::Tensor x, torch::Tensor gate,
+                                          c10::optional<torch::Tensor> state,
+                                          c10::optional<torch::Tensor> lens,
+                                          bool reverse, std::string act,
+                                          bool want_bnd);
+torch::Tensor gated_scan_bwd(torch::Tensor x, torch::Tensor gate,
+                             c10::optional<torch::Tensor> state,
+                             c10::optional<torch::Tensor> lens,
+                             torch::Tensor bnd,
+                             c10::optional<torch::Tensor> dy,
+                             c10::optional<torch::Tensor> dlast, bool reverse,
+                             std::string act, torch::Tensor dx,
+                             torch::Tensor dgate, bool want_dstate);
+torch::Tensor gated_step(torch::Tensor x, torch::Tensor gate,
+                         torch::Tensor state, torch::Tensor state_out,
+                         std::string act);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layernorm_fwd", &layernorm_fwd, "LayerNorm forward (gfx950)");
   m.def("layernorm_res_fwd", &layernorm_res_fwd,
@@ -98,4 +115,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sumsq_finite", &sumsq_finite, "fused grad sumsq + nonfinite count");
   m.def("beam_topk", &beam_topk,
         "fused beam-search top-k (path-score add + UNK suppression)");
+  m.def("gated_scan_fwd", &gated_scan_fwd,
+        "gated linear recurrence over sequences");
+  m.def("gated_scan_bwd", &gated_scan_bwd,
+        "its gradient, written into given strided views");
+  m.def("gated_step", &gated_step,
+        "gated linear recurrence, one token per row");
 }

@@ -35,6 +35,9 @@ if os.path.exists(colsum):
 fp8q = os.path.join(HIP_DIR, "fp8q.hip")
 if os.path.exists(fp8q):
     sources.append(fp8q)
+for name in ("gated_scan.hip", "block_norm.hip"):
+    if os.path.exists(os.path.join(HIP_DIR, name)):
+        sources.append(os.path.join(HIP_DIR, name))
 ltgemm = os.path.join(HIP_DIR, "ltgemm.cpp")
 if os.path.exists(ltgemm):
     sources.append(ltgemm)
@@ -45,7 +48,9 @@ ext = CUDAExtension(
     libraries=["hipblaslt"],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],
-        "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950"],
+        # no packed fp32 instructions: some of their forms are not reliable
+        "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950", "-Xclang",
+                 "-target-feature", "-Xclang", "-packed-fp32-ops"],
     },
 )
 

@@ -1,0 +1,400 @@
+"""Gated linear recurrence (ops.gated_scan, gated_scan_xg, gated_step) against
+the recurrence and its gradient written out step by step in 64 bits.
+
+Tolerances. With u = 2^-24 one step  c = f c' + om x  has an error of at most
+(e_f + e_om + 3) u amax, where the sigmoid's parts are good to e = |g| + 3
+units (its exponential's argument is rounded once, exp, sum and reciprocal
+add one unit each); earlier errors are multiplied by f <= 1, and joining runs
+of steps costs a product and a sum per join, at most one join per step. So T
+steps stay within K u amax with K = T (4 gmax + 32), amax the largest |x| or
+|state|. The gradient's recurrence is the same one, over lam; dg multiplies
+lam, c - x and f om <= 1/4. The last rounding to the output's type adds
+eps / 2 of the value.
+"""
+import pytest
+import torch
+
+from marian_amd import ops
+
+U = 2.0 ** -24
+
+
+def oracle(x, g, state, lens, reverse, act, dy, dlast):
+    """All results in float64, and the largest |lam|."""
+    x, g, dy = x.double().cpu(), g.double().cpu(), dy.double().cpu()
+    B, T, D = x.shape
+    c = torch.zeros(B, D, dtype=torch.float64) if state is None \
+        else state.double().cpu()
+    lam_in = dlast.double().cpu().clone()
+    y, dx, dg = (torch.zeros_like(x) for _ in range(3))
+    dstate = torch.zeros(B, D, dtype=torch.float64)
+    last = c.clone()
+    lmax, cmin = float(lam_in.abs().max()) if lam_in.numel() else 0.0, 1e9
+    for b in range(B):
+        n = T if lens is None else min(max(int(lens[b]), 0), T)
+        order = list(range(n))[::-1] if reverse else list(range(n))
+        cur, prevs = c[b].clone(), []
+        for t in order:
+            f = 1 / (1 + torch.exp(-g[b, t]))
+            prevs.append(cur)
+            cur = f * cur + (1 - f) * x[b, t]
+            y[b, t] = torch.where(cur < 0, 0 * cur, cur) if act == "relu" \
+                else cur
+            if act == "relu":
+                cmin = min(cmin, float(cur.abs().min()))
+        last[b] = cur
+        mu = lam_in[b].clone()
+        for t, prev in zip(order[::-1], prevs[::-1]):
+            f = 1 / (1 + torch.exp(-g[b, t]))
+            now = f * prev + (1 - f) * x[b, t]
+            d = torch.where(now > 0, dy[b, t], 0 * now) if act == "relu" \
+                else dy[b, t]
+            lam = d + mu
+            lmax = max(lmax, float(lam.abs().max()))
+            dx[b, t] = (1 - f) * lam
+            dg[b, t] = f * (1 - f) * (prev - x[b, t]) * lam
+            mu = f * lam
+        dstate[b] = mu
+    return y, last, dx, dg, dstate, lmax, cmin
+
+
+def close(got, want, atol, dtype):
+    half = torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -7)
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape
+    err = (got - want).abs()
+    lim = atol + half * (want.abs() + atol)
+    assert bool((err <= lim).all()), \
+        f"off by {float((err - lim).max())} over the limit"
+
+
+def make(B, T, D, dtype, dev, seed, state=True, lens=None):
+    gen = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=gen)
+    xg = torch.cat([r(B, T, D), r(B, T, D) * 2 + 0.5], -1).to(dtype).to(dev)
+    sdt = torch.float64 if dtype == torch.float64 else torch.float32
+    st = r(B, D).to(sdt).to(dev) if state else None
+    ln = None
+    if lens == "ragged":
+        ln = torch.randint(0, T + 1, (B,), generator=gen).to(torch.int32)
+        ln[0] = 0
+        if B > 1:
+            ln[1] = T
+        ln = ln.to(dev)
+    dy = r(B, T, D).to(dtype).to(dev)
+    dlast = r(B, D).to(sdt).to(dev)
+    return xg, st, ln, dy, dlast
+
+
+def check_case(dev, B, T, D, dtype, lens=None, reverse=False, act="none",
+               state=True, layout="split", seed=0):
+    # relu's side must not be a matter of rounding: the first inputs whose
+    # states, by the oracle, all stay further from 0 than the tolerance
+    for seed in range(seed, seed + 200):
+        xg, st, ln, dy, dlast = make(B, T, D, dtype, dev, seed, state, lens)
+        want = oracle(xg[..., :D], xg[..., D:], st, ln, reverse, act, dy,
+                      dlast)
+        gmax = float(xg[..., D:].abs().max()) if xg.numel() else 0.0
+        K = max(T, 1) * (4 * gmax + 32) * U
+        amax = float(xg[..., :D].abs().max()) if xg.numel() else 0.0
+        if st is not None:
+            amax = max(amax, float(st.abs().max()))
+        if want[6] > K * amax:
+            break
+    assert want[6] > K * amax
+    if st is not None:
+        st.requires_grad_()
+    kw = dict(state=st, lens=ln, reverse=reverse, act=act)
+    if layout == "fused":
+        xg.requires_grad_()
+        leaves = [xg]
+        y, last = ops.gated_scan_xg(xg, **kw)
+    else:
+        if layout == "views":       # halves of one buffer, transposed batch
+            buf = xg.transpose(0, 1).contiguous().transpose(0, 1)
+            x, g = buf[..., :D], buf[..., D:]
+        else:
+            x, g = xg[..., :D].contiguous(), xg[..., D:].contiguous()
+        if layout == "columns":     # the last dimension is not dense
+            x = x.transpose(1, 2).contiguous().transpose(1, 2)
+        x, g = x.detach().requires_grad_(), g.detach().requires_grad_()
+        leaves = [x, g]
+        y, last = ops.gated_scan(x, g, **kw)
+    assert y.dtype == dtype and y.is_contiguous()
+    if st is not None:
+        leaves.append(st)
+    grads = torch.autograd.grad((y, last), leaves, (dy, dlast))
+    if layout == "fused":
+        grads = (grads[0][..., :D], grads[0][..., D:]) + grads[1:]
+    sdt = last.dtype
+    lmax = want[5]
+    close(y, want[0], K * amax, dtype)
+    close(last, want[1], K * amax, sdt)
+    close(grads[0], want[2], K * lmax, dtype)
+    close(grads[1], want[3], K * lmax * 2 * amax, dtype)
+    if st is not None:
+        close(grads[2], want[4], K * lmax, sdt)
+
+
+CPU_CASES = [
+    dict(B=2, T=5, D=3, dtype=torch.float32),
+    dict(B=3, T=9, D=4, dtype=torch.float32, lens="ragged", reverse=True),
+    dict(B=2, T=7, D=5, dtype=torch.bfloat16, act="relu", layout="fused"),
+    dict(B=2, T=1, D=2, dtype=torch.float64, state=False),
+    dict(B=1, T=0, D=2, dtype=torch.float32),
+]
+
+
+@pytest.mark.parametrize("case", CPU_CASES)
+def test_scan_plain_matches_oracle(case):
+    check_case("cpu", **case)
+
+
+def test_scan_plain_gradients_by_differences():
+    xg, st, ln, _, _ = make(2, 6, 3, torch.float64, "cpu", 3, True, "ragged")
+    xg.requires_grad_()
+    st.requires_grad_()
+    for rev in (False, True):
+        assert torch.autograd.gradcheck(
+            lambda a, s: ops.gated_scan_xg(a, s, ln, rev), (xg, st))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_step_walks_like_the_scan(dtype):
+    xg, st, _, dy, dl = make(3, 5, 7, dtype, "cpu", 4)
+    y, last = ops.gated_scan_xg(xg, st, act="relu")
+    want = oracle(xg[..., :7], xg[..., 7:], st, None, False, "relu", dy, dl)
+    lim = 5 * (4 * float(xg[..., 7:].abs().max()) + 32) * U \
+        * max(float(xg[..., :7].abs().max()), float(st.abs().max()))
+    close(y, want[0], lim, dtype)
+    cur = st.clone()
+    for t in range(5):
+        o, new = ops.gated_step(xg[:, t, :7], xg[:, t, 7:], cur, act="relu",
+                                inplace=True)
+        assert new is cur
+        close(o, want[0][:, t], lim, dtype)
+    close(last, want[1], lim, torch.float32)
+    close(cur, want[1], lim, torch.float32)
+
+
+def test_step_gradient_is_the_scans():
+    xg, st, _, _, _ = make(3, 1, 4, torch.float64, "cpu", 5)
+    xg.requires_grad_()
+    st.requires_grad_()
+    assert torch.autograd.gradcheck(
+        lambda a, s: ops.gated_step(a[:, 0, :4], a[:, 0, 4:], s), (xg, st))
+
+
+def _refused(fn, *a, **k):
+    with pytest.raises(ValueError):
+        fn(*a, **k)
+
+
+def test_scan_refusals():
+    x = torch.zeros(2, 3, 4)
+    s = torch.zeros(2, 4)
+    _refused(ops.gated_scan, x[0], x[0])
+    _refused(ops.gated_scan, x, x[:, :2])
+    _refused(ops.gated_scan, x, x.bfloat16())
+    _refused(ops.gated_scan, x.long(), x.long())
+    _refused(ops.gated_scan, x[..., :0], x[..., :0])
+    _refused(ops.gated_scan, x, x, act="tanh")
+    _refused(ops.gated_scan, x, x, state=s.bfloat16())
+    _refused(ops.gated_scan, x, x, state=s[:1])
+    _refused(ops.gated_scan, x, x, lens=torch.zeros(2))
+    _refused(ops.gated_scan, x, x, lens=torch.zeros(3, dtype=torch.int32))
+    _refused(ops.gated_scan, x, x, lens=torch.zeros(2, dtype=torch.int64))
+    _refused(ops.gated_scan_xg, x[..., :3])
+    _refused(ops.gated_scan_xg, x[0])
+
+
+def test_step_refusals():
+    x, s = torch.zeros(2, 4), torch.zeros(2, 4)
+    _refused(ops.gated_step, x, x, None)
+    _refused(ops.gated_step, x[:, None], x[:, None], s)
+    _refused(ops.gated_step, x, x, s[:1])
+    _refused(ops.gated_step, x, x, s.half())
+    _refused(ops.gated_step, x, x, torch.zeros(4, 2).t(), inplace=True)
+    _refused(ops.gated_step, x.requires_grad_(), x, s, inplace=True)
+
+
+# ------------------------------------------------------------------ on the GPU
+
+GPU_CASES = [
+    dict(B=1, T=1, D=1, dtype=torch.float32),
+    dict(B=2, T=1, D=3, dtype=torch.bfloat16, state=False),
+    dict(B=1, T=0, D=8, dtype=torch.float32),
+    dict(B=3, T=2, D=2, dtype=torch.float16),
+    dict(B=2, T=63, D=5, dtype=torch.float32, lens="ragged"),
+    dict(B=2, T=64, D=64, dtype=torch.bfloat16, layout="fused"),
+    dict(B=2, T=65, D=257, dtype=torch.float16, layout="views"),
+    dict(B=3, T=66, D=30, dtype=torch.float32, layout="columns"),
+    dict(B=4, T=130, D=509, dtype=torch.float32, lens="ragged", reverse=True),
+    dict(B=5, T=200, D=33, dtype=torch.bfloat16, lens="ragged", reverse=True,
+         layout="fused"),
+    dict(B=1, T=1000, D=70, dtype=torch.float32, reverse=True),
+    dict(B=1, T=1025, D=256, dtype=torch.bfloat16, layout="fused"),
+    dict(B=2, T=40, D=6, dtype=torch.float32, act="relu", lens="ragged"),
+    dict(B=2, T=40, D=6, dtype=torch.float32, act="relu", reverse=True),
+    dict(B=300, T=3, D=17, dtype=torch.float16, lens="ragged"),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", GPU_CASES)
+def test_scan_gpu_matches_oracle(case):
+    check_case("cuda", **case)
+
+
+@pytest.mark.gpu
+def test_scan_gpu_padded_values_are_ignored():
+    """NaN and infinities behind the sequences, in inputs and gradients."""
+    for rev in (False, True):
+        xg, st, ln, dy, dlast = make(4, 70, 24, torch.float32, "cuda", 7, True,
+                                     "ragged")
+        pad = (torch.arange(70, device="cuda")[None] >= ln[:, None])[..., None]
+        bad = torch.where(pad, float("nan"), xg).requires_grad_()
+        good = xg.clone().requires_grad_()
+        st.requires_grad_()
+        outs = []
+        for a, d in ((good, dy), (bad, torch.where(pad, float("inf"), dy))):
+            y, last = ops.gated_scan_xg(a, st, ln, rev)
+            outs.append((y, last) + torch.autograd.grad((y, last), (a, st),
+                                                        (d, dlast)))
+        for p, q in zip(*outs):
+            assert torch.equal(p, q)
+        assert bool((outs[1][0] * pad == 0).all())
+        assert bool((outs[1][2] * pad == 0).all())
+
+
+@pytest.mark.gpu
+def test_scan_gpu_extreme_gates_and_nan():
+    """Infinite gate logits keep or replace the state; NaN stays in its
+    channel and is not hidden by relu."""
+    x = torch.randn(1, 4, 8, device="cuda")
+    g = torch.full_like(x, float("inf"))
+    st = torch.randn(1, 8, device="cuda")
+    y, last = ops.gated_scan(x, g, st)
+    assert torch.equal(last, st) and torch.equal(y, st[:, None].expand_as(y))
+    y, last = ops.gated_scan(x, -g, st)
+    assert torch.equal(y, x) and torch.equal(last, x[:, -1])
+    x[0, 1, 3] = float("nan")
+    y, last = ops.gated_scan(x, torch.zeros_like(x), st, act="relu")
+    want = torch.zeros(1, 4, 8, dtype=torch.bool, device="cuda")
+    want[0, 1:, 3] = True
+    assert torch.equal(torch.isnan(y), want)
+
+
+@pytest.mark.gpu
+def test_scan_gpu_partial_gradients():
+    """Only one of the outputs is used; only one of the inputs wants one."""
+    xg, st, _, dy, dlast = make(2, 70, 12, torch.float32, "cuda", 8)
+    x, g = xg[..., :12].contiguous(), xg[..., 12:].contiguous()
+    x.requires_grad_(), g.requires_grad_(), st.requires_grad_()
+    zl, zy = torch.zeros_like(dlast), torch.zeros_like(dy)
+    a = torch.autograd.grad(ops.gated_scan(x, g, st)[0], (x, g, st), dy)
+    b = torch.autograd.grad(ops.gated_scan(x, g, st), (x, g, st), (dy, zl))
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    a = torch.autograd.grad(ops.gated_scan(x, g, st)[1], (x, g, st), dlast)
+    b = torch.autograd.grad(ops.gated_scan(x, g, st), (x, g, st), (zy, dlast))
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    a = torch.autograd.grad(ops.gated_scan(x.detach(), g, st.detach())[0], g,
+                            dy.expand_as(dy))
+    b = torch.autograd.grad(ops.gated_scan(x, g, st)[0], g, dy)
+    assert torch.equal(a[0], b[0])
+    # a gradient that is broadcast, as sum() gives
+    a = torch.autograd.grad(ops.gated_scan(x, g)[0].sum(), x)
+    b = torch.autograd.grad(ops.gated_scan(x, g)[0], x, torch.ones_like(dy))
+    assert torch.equal(a[0], b[0])
+
+
+@pytest.mark.gpu
+def test_scan_gpu_repeats_bit_for_bit():
+    xg, st, ln, dy, dlast = make(3, 700, 40, torch.bfloat16, "cuda", 9, True,
+                                 "ragged")
+    xg.requires_grad_(), st.requires_grad_()
+
+    def once():
+        o = ops.gated_scan_xg(xg, st, ln, True)
+        return o + torch.autograd.grad(o, (xg, st), (dy, dlast))
+    first = once()
+    for _ in range(3):
+        assert all(torch.equal(p, q) for p, q in zip(first, once()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16,
+                                   torch.float16])
+@pytest.mark.parametrize("N,D", [(1, 1), (3, 5), (4, 64), (7, 1023),
+                                 (130, 6)])
+@pytest.mark.parametrize("inplace", [False, True])
+def test_step_gpu(dtype, N, D, inplace):
+    xg, st, _, dy, dlast = make(N, 1, D, dtype, "cuda", N + D)
+    want = oracle(xg[..., :D], xg[..., D:], st, None, False, "relu", dy, dlast)
+    K = (4 * float(xg[..., D:].abs().max()) + 32) * U
+    amax = max(float(xg[..., :D].abs().max()), float(st.abs().max()))
+    before = st.clone()
+    y, new = ops.gated_step(xg[:, 0, :D], xg[:, 0, D:], st, act="relu",
+                            inplace=inplace)
+    assert (new is st) == inplace
+    if not inplace:
+        assert torch.equal(st, before)
+    close(y, want[0][:, 0], K * amax, dtype)
+    close(new, want[1], K * amax, torch.float32)
+
+
+@pytest.mark.gpu
+def test_step_gpu_captured():
+    """An in-place step replayed from a graph advances the state each time,
+    as eager steps on another stream do."""
+    xg, st, _, _, _ = make(5, 6, 48, torch.bfloat16, "cuda", 11)
+    y, last = ops.gated_scan_xg(xg, st)
+    tok = xg[:, 0].clone()
+    state = st.clone()
+    ops.gated_step(tok[:, :48], tok[:, 48:], state.clone(), inplace=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, _ = ops.gated_step(tok[:, :48], tok[:, 48:], state, inplace=True)
+    side = torch.cuda.Stream()
+    eager = st.clone()
+    side.wait_stream(torch.cuda.current_stream())
+    for t in range(6):
+        tok.copy_(xg[:, t])
+        graph.replay()
+        with torch.cuda.stream(side):
+            ye, eager = ops.gated_step(xg[:, t, :48], xg[:, t, 48:], eager)
+        torch.cuda.synchronize()
+        assert torch.equal(out, ye) and torch.equal(state, eager)
+    close(state, last.double().cpu(), 6 * 80 * U * 4, torch.float32)
+
+
+@pytest.mark.gpu
+def test_scan_gpu_captured():
+    """Forward and backward replayed from two graphs that interleave."""
+    graphs = []
+    for seed in (1, 2):
+        xg, st, ln, dy, dlast = make(2, 900, 64, torch.bfloat16, "cuda", seed,
+                                     True, "ragged")
+        xg.requires_grad_(), st.requires_grad_()
+
+        def once(a=xg, s=st, n=ln, d=(dy, dlast)):
+            o = ops.gated_scan_xg(a, s, n)
+            return [t.detach() for t in o] + list(
+                torch.autograd.grad(o, (a, s), d))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            once()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = once()
+        graphs.append((graph, outs, once))
+    for _ in range(3):
+        for graph, outs, _ in graphs:
+            for o in outs:
+                o.zero_()
+        for graph, _, _ in graphs:
+            graph.replay()
+        for _, outs, once in graphs:
+            assert all(torch.equal(p, q) for p, q in zip(outs, once()))
