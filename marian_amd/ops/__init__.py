@@ -238,6 +238,56 @@ def layer_norm_residual(x: torch.Tensor, res: torch.Tensor,
 
 
 # ---------------------------------------------------------------------------
+# The join of two transformer blocks (ref: transformer.h pre/postProcess)
+# ---------------------------------------------------------------------------
+
+def block_norm(x: torch.Tensor, res: torch.Tensor,
+               gate: Optional[torch.Tensor] = None, gate_kind: str = "scale",
+               res_scale: float = 1.0,
+               post_scale: Optional[torch.Tensor] = None,
+               post_bias: Optional[torch.Tensor] = None,
+               pre_scale: Optional[torch.Tensor] = None,
+               pre_bias: Optional[torch.Tensor] = None,
+               norm: str = "layer", eps: float = 1e-9):
+    """A block's output norm, gate and residual sum, and the norm before the
+    next block; returns (s, h), h None without pre_scale.
+
+        u = norm(x; post_scale, post_bias)   or x without post_scale
+        s = res_scale * res + u                                 no gate
+        s = res_scale * res + gate * u                          "scale"
+        s = res_scale * (1 - k) * res + k * u, k = sigmoid(gate)  "highway"
+        h = norm(s; pre_scale, pre_bias)
+
+    norm: "layer" ((v - mean) / sqrt(var + eps)) or "rms" (v / sqrt(mean v^2
+    + eps)), times scale, plus bias if there is one. x, res: [..., D], fp32 /
+    bf16 / fp16, D <= 16384. gate: [D] (per channel) or x's shape (per
+    token). Parameters are [D], all of x's dtype or all float32. h is taken
+    from the 32-bit s; s and h are rounded once. Differentiable once in every
+    tensor.
+    """
+    from ._block_norm import BlockNormFn, block_norm_torch, check_join
+    check_join(x, res, gate, gate_kind,
+               {"post_scale": post_scale, "post_bias": post_bias,
+                "pre_scale": pre_scale, "pre_bias": pre_bias}, norm)
+    if not _on_gpu(x):
+        return block_norm_torch(x, res, gate, gate_kind, res_scale,
+                                post_scale, post_bias, pre_scale, pre_bias,
+                                norm, eps)
+    D = x.shape[-1]
+    if gate is not None and (gate.dim() > 1 or x.dim() == 1):
+        gate = gate.reshape(-1, D).contiguous()
+    vec = [None if v is None else v.contiguous()
+           for v in (post_scale, post_bias, pre_scale, pre_bias)]
+    if gate is not None and gate.dim() == 1:
+        gate = gate.contiguous()
+    s, h = BlockNormFn.apply(
+        x.reshape(-1, D).contiguous(), res.reshape(-1, D).contiguous(), gate,
+        *vec, gate_kind == "highway", float(res_scale), norm == "rms",
+        float(eps))
+    return s.view(x.shape), h.view(x.shape) if pre_scale is not None else None
+
+
+# ---------------------------------------------------------------------------
 # Gated linear recurrence (ref: rnn/cells.h SSRU)
 # ---------------------------------------------------------------------------
 

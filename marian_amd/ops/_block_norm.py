@@ -1,0 +1,115 @@
+"""The join of two transformer blocks (norm, gate, residual, next norm):
+argument checks, the autograd wrapper of the HIP kernels and the plain
+composite used off the GPU.
+
+ref: models/transformer.h preProcess/postProcess ('n', 'a') and the highway
+functor (out = sigmoid(t) in1 + (1 - sigmoid(t)) in2).
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import hip_ext
+
+MAX_WIDTH = 16384
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def check_join(x, res, gate, gate_kind, params, norm):
+    """params: {name: tensor or None} of the four norm parameters."""
+    ok = _DTYPES if x.is_cuda else _DTYPES + (torch.float64,)
+    if x.dim() < 1 or x.dtype not in ok:
+        raise ValueError(f"block_norm: x must be [..., D] of {ok}, got "
+                         f"{x.dtype} {tuple(x.shape)}")
+    D = x.shape[-1]
+    if not 0 < D <= MAX_WIDTH:
+        raise ValueError(f"block_norm: the width must be 1..{MAX_WIDTH}, "
+                         f"got {D}")
+    if res.shape != x.shape or res.dtype != x.dtype \
+            or res.device != x.device:
+        raise ValueError("block_norm: res must have x's shape, dtype and "
+                         "device")
+    if norm not in ("layer", "rms"):
+        raise ValueError(f"block_norm: norm must be layer or rms, got "
+                         f"{norm!r}")
+    if gate_kind not in ("scale", "highway"):
+        raise ValueError("block_norm: gate_kind must be scale or highway, "
+                         f"got {gate_kind!r}")
+    vecs = {k: v for k, v in params.items() if v is not None}
+    if gate is not None:
+        if gate.dim() == 1 and gate.shape == (D,) and x.dim() > 1:
+            vecs["gate"] = gate
+        elif gate.shape != x.shape or gate.dtype != x.dtype \
+                or gate.device != x.device:
+            raise ValueError("block_norm: gate must be [D] or of x's shape "
+                             f"and dtype, got {gate.dtype} "
+                             f"{tuple(gate.shape)}")
+    for side in ("post", "pre"):
+        if params[side + "_bias"] is not None \
+                and params[side + "_scale"] is None:
+            raise ValueError(f"block_norm: {side}_bias needs {side}_scale")
+    pdt = {v.dtype for v in vecs.values()}
+    if len(pdt) > 1 or not pdt <= {x.dtype, torch.float32}:
+        raise ValueError("block_norm: parameters must share one dtype, "
+                         f"x's or float32, got {sorted(map(str, pdt))}")
+    for k, v in vecs.items():
+        if v.shape != (D,) or v.device != x.device:
+            raise ValueError(f"block_norm: {k} must be [{D}] on x's device")
+
+
+def block_norm_torch(x, res, gate=None, gate_kind="scale", res_scale=1.0,
+                     post_scale=None, post_bias=None, pre_scale=None,
+                     pre_bias=None, norm="layer", eps=1e-9):
+    """The formulas in (at least) 32 bits."""
+    acc = torch.float64 if x.dtype == torch.float64 else torch.float32
+
+    def normed(v, scale, bias):
+        if norm == "layer":
+            v = v - v.mean(-1, keepdim=True)
+        v = v * torch.rsqrt((v * v).mean(-1, keepdim=True) + eps)
+        v = v * scale.to(acc)
+        return v if bias is None else v + bias.to(acc)
+
+    u, r = x.to(acc), res.to(acc) * res_scale
+    if post_scale is not None:
+        u = normed(u, post_scale, post_bias)
+    if gate is None:
+        s = r + u
+    elif gate_kind == "scale":
+        s = r + gate.to(acc) * u
+    else:
+        g = gate.to(acc)
+        s = torch.sigmoid(-g) * r + torch.sigmoid(g) * u
+    h = None if pre_scale is None else normed(s, pre_scale, pre_bias).to(
+        x.dtype)
+    return s.to(x.dtype), h
+
+
+class BlockNormFn(torch.autograd.Function):
+    """x and res as [R, D]; returns (s, h) with h empty without pre_scale."""
+
+    @staticmethod
+    def forward(ctx, x, res, gate, post_scale, post_bias, pre_scale, pre_bias,
+                highway, alpha, rms, eps):
+        want = any(ctx.needs_input_grad)
+        s, h, stat = hip_ext(required=True).block_norm_fwd(
+            x, res, gate, highway, alpha, post_scale, post_bias, pre_scale,
+            pre_bias, rms, eps, want)
+        if want:
+            ctx.save_for_backward(x, res, gate, post_scale, post_bias,
+                                  pre_scale, pre_bias, stat)
+            ctx.conf = (highway, alpha, rms, eps)
+            ctx.set_materialize_grads(False)
+        return s, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, ds, dh):
+        x, res, gate, w1, b1, w2, b2, stat = ctx.saved_tensors
+        highway, alpha, rms, eps = ctx.conf
+        want = list(ctx.needs_input_grad[:7])
+        outs = hip_ext(required=True).block_norm_bwd(
+            x, res, gate, highway, alpha, w1, b1, w2, b2, rms, eps, stat, ds,
+            dh, want)
+        return tuple(o if w else None for o, w in zip(outs, want)) + (None,) * 4

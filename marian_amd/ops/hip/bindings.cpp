@@ -72,6 +72,21 @@ torch::Tensor gated_scan_bwd(torch::Tensor x, torch::Tensor gate,
 torch::Tensor gated_step(torch::Tensor x, torch::Tensor gate,
                          torch::Tensor state, torch::Tensor state_out,
                          std::string act);
+std::vector<torch::Tensor> block_norm_fwd(
+    torch::Tensor x, torch::Tensor res, c10::optional<torch::Tensor> gate,
+    bool highway, double alpha, c10::optional<torch::Tensor> post_scale,
+    c10::optional<torch::Tensor> post_bias,
+    c10::optional<torch::Tensor> pre_scale,
+    c10::optional<torch::Tensor> pre_bias, bool rms, double eps,
+    bool want_stat);
+std::vector<torch::Tensor> block_norm_bwd(
+    torch::Tensor x, torch::Tensor res, c10::optional<torch::Tensor> gate,
+    bool highway, double alpha, c10::optional<torch::Tensor> post_scale,
+    c10::optional<torch::Tensor> post_bias,
+    c10::optional<torch::Tensor> pre_scale,
+    c10::optional<torch::Tensor> pre_bias, bool rms, double eps,
+    torch::Tensor stat, c10::optional<torch::Tensor> dsum,
+    c10::optional<torch::Tensor> dh, std::vector<bool> want);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layernorm_fwd", &layernorm_fwd, "LayerNorm forward (gfx950)");
@@ -121,4 +136,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "its gradient, written into given strided views");
   m.def("gated_step", &gated_step,
         "gated linear recurrence, one token per row");
+  m.def("block_norm_fwd", &block_norm_fwd,
+        "fused norm, gate, residual and next norm of a block");
+  m.def("block_norm_bwd", &block_norm_bwd, "its gradient");
 }

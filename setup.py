@@ -35,7 +35,8 @@ if os.path.exists(colsum):
 fp8q = os.path.join(HIP_DIR, "fp8q.hip")
 if os.path.exists(fp8q):
     sources.append(fp8q)
-for name in ("gated_scan.hip", "block_norm.hip"):
+for name in ("gated_scan.hip", "block_norm.hip", "block_norm_bf16.hip",
+             "block_norm_f16.hip", "block_norm_f32.hip"):
     if os.path.exists(os.path.join(HIP_DIR, name)):
         sources.append(os.path.join(HIP_DIR, name))
 ltgemm = os.path.join(HIP_DIR, "ltgemm.cpp")
@@ -45,6 +46,8 @@ if os.path.exists(ltgemm):
 ext = CUDAExtension(
     name="marian_amd.ops._hip_ext",
     sources=sources,
+    depends=[os.path.join(HIP_DIR, name)
+             for name in ("common.h", "vec.h", "block_norm.h")],
     libraries=["hipblaslt"],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],

@@ -1,0 +1,373 @@
+"""The fused block join (ops.block_norm) against its formulas and gradients in
+64 bits.
+
+Tolerances come from a running error bound: the oracle carries, beside every
+64-bit value, how far 32-bit arithmetic with unit u = 2^-24 may be from it
+(sums and products add u of their result to what their operands bring, a mean
+over a row 32 u of the mean of absolute values - a lane adds at most 16
+elements, a wave joins in 6 steps and a row's waves in at most 16 - and a sum
+over rows 128 u of the sum of absolute values). Twice that bound covers the
+order of the operations, and the last rounding adds eps / 2 of the value.
+"""
+import pytest
+import torch
+
+from marian_amd import ops
+
+U = 2.0 ** -24
+
+
+class Num:
+    """A 64-bit value and the bound on a 32-bit computation's error."""
+
+    def __init__(self, v, e=None):
+        self.v, self.e = v, torch.zeros_like(v) if e is None else e
+
+    def _out(self, v, e):
+        return Num(v, e + U * (v.abs() + e))
+
+    def __add__(self, o):
+        return self._out(self.v + o.v, self.e + o.e)
+
+    def __sub__(self, o):
+        return self._out(self.v - o.v, self.e + o.e)
+
+    def __mul__(self, o):
+        return self._out(self.v * o.v, self.v.abs() * o.e
+                         + o.v.abs() * self.e + self.e * o.e)
+
+    def times(self, c):
+        return self._out(self.v * c, self.e * abs(c))
+
+    def mean(self):
+        return Num(self.v.mean(-1, keepdim=True),
+                   self.e.mean(-1, keepdim=True)
+                   + 32 * U * self.v.abs().mean(-1, keepdim=True))
+
+    def rows(self):
+        return Num(self.v.sum(0),
+                   self.e.sum(0) + 128 * U * self.v.abs().sum(0))
+
+    def rsqrt(self, eps):
+        x = self.v + eps
+        r = x.rsqrt()
+        # the error of x, when it is small beside x, halves; floor at 0
+        lo = (x - self.e - U * x).clamp_min(eps / 2)
+        return Num(r, (lo.rsqrt() - r) + 3 * U * r)
+
+    def sigmoid(self):
+        v = torch.sigmoid(self.v)
+        return Num(v, v * (2 * self.v.abs() + 6) * U)
+
+
+def oracle(t, norm, gate_kind, alpha, eps=1e-9):
+    d = {k: None if v is None else Num(v.detach().double().cpu())
+         for k, v in t.items()}
+
+    def normed(v, side):
+        if norm == "layer":
+            v = v - v.mean()
+        r = (v * v).mean().rsqrt(eps)
+        xh = v * r
+        y = xh * d[side + "_scale"]
+        return (y if d[side + "_bias"] is None else y + d[side + "_bias"]), \
+            xh, r
+
+    def norm_grad(g, xh, r):
+        o = g - xh * (g * xh).mean()
+        return (o - g.mean() if norm == "layer" else o) * r
+
+    x, res = d["x"], d["res"]
+    u, xh, xr = normed(x, "post") if d["post_scale"] is not None \
+        else (x, None, None)
+    one = Num(torch.ones(1, dtype=torch.float64))
+    ca, cb, k, k1 = one.times(alpha), one, None, None
+    if d["gate"] is not None:
+        if gate_kind == "highway":
+            k, k1 = d["gate"].sigmoid(), Num(-d["gate"].v).sigmoid()
+            ca, cb = k1.times(alpha), k
+        else:
+            cb = d["gate"]
+    s = ca * res + cb * u
+    out = {"s": s}
+    ds = d["dsum"]
+    if d["pre_scale"] is not None:
+        out["h"], sh, sr = normed(s, "pre")
+        dh = d["dh"]
+        out["pre_scale"], out["pre_bias"] = (dh * sh).rows(), dh.rows()
+        ds = ds + norm_grad(dh * d["pre_scale"], sh, sr)
+    out["res"] = ca * ds
+    du = cb * ds
+    if d["gate"] is not None:
+        g = u * ds if gate_kind == "scale" else \
+            k * k1 * (u - res.times(alpha)) * ds
+        out["gate"] = g.rows() if d["gate"].v.dim() == 1 else g
+    out["x"] = du
+    if d["post_scale"] is not None:
+        out["post_scale"], out["post_bias"] = (du * xh).rows(), du.rows()
+        out["x"] = norm_grad(du * d["post_scale"], xh, xr)
+    return out
+
+
+LEAVES = ("x", "res", "gate", "post_scale", "post_bias", "pre_scale",
+          "pre_bias")
+
+
+def make(R, D, dtype, dev, norm="layer", gate=None, per_token=False, post=True,
+         pre=True, bias=True, pdt=None, seed=0, shift=0.5):
+    gen = torch.Generator().manual_seed(seed)
+    rnd = lambda *s: torch.randn(*s, generator=gen)
+    pdt = pdt or dtype
+    t = {"x": (rnd(R, D) * 2 + shift).to(dtype),
+         "res": (rnd(R, D) * 3 - 0.5).to(dtype), "gate": None,
+         "dsum": rnd(R, D).to(dtype),
+         "dh": rnd(R, D).to(dtype) if pre else None}
+    if gate:
+        t["gate"] = (rnd(R, D) if per_token else rnd(D)).add(0.3).to(
+            dtype if per_token else pdt)
+    for side, on in (("post", post), ("pre", pre)):
+        t[side + "_scale"] = (1 + 0.2 * rnd(D)).to(pdt) if on else None
+        t[side + "_bias"] = (0.3 * rnd(D)).to(pdt) \
+            if on and bias and norm == "layer" else None
+    return {k: None if v is None else v.to(dev) for k, v in t.items()}
+
+
+def close(name, got, want, dtype):
+    assert got.dtype == dtype and got.shape == want.v.shape, name
+    half = torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -7)
+    err = (got.detach().double().cpu() - want.v).abs()
+    # below the normal range a half step is absolute
+    lim = 2 * want.e + half * (want.v.abs() + 2 * want.e) \
+        + torch.finfo(dtype).smallest_normal * half
+    assert bool((err <= lim).all()), \
+        f"{name}: off by {float((err - lim).max())} over the limit"
+
+
+def call(t, norm, gate_kind, alpha):
+    return ops.block_norm(t["x"], t["res"], t["gate"], gate_kind, alpha,
+                          t["post_scale"], t["post_bias"], t["pre_scale"],
+                          t["pre_bias"], norm)
+
+
+def run(t, norm, gate_kind, alpha):
+    leaves = [k for k in LEAVES if t[k] is not None]
+    for k in leaves:
+        t[k].requires_grad_()
+    s, h = call(t, norm, gate_kind, alpha)
+    outs = [s] + ([h] if h is not None else [])
+    grads = torch.autograd.grad(outs, [t[k] for k in leaves],
+                                [t["dsum"], t["dh"]][:len(outs)])
+    return s, h, dict(zip(leaves, grads))
+
+
+def check_case(dev, R, D, dtype, norm="layer", gate=None, alpha=1.0, **kw):
+    t = make(R, D, dtype, dev, norm=norm, gate=gate, **kw)
+    s, h, grads = run(t, norm, gate or "scale", alpha)
+    want = oracle(t, norm, gate, alpha)
+    close("s", s, want["s"], dtype)
+    assert (h is None) == (t["pre_scale"] is None)
+    if h is not None:
+        close("h", h, want["h"], dtype)
+    for k, g in grads.items():
+        close(k, g, want[k], t[k].dtype)
+
+
+CPU_CASES = [
+    dict(R=3, D=8, dtype=torch.float32),
+    dict(R=3, D=5, dtype=torch.float32, norm="rms", gate="scale", alpha=0.5),
+    dict(R=4, D=16, dtype=torch.bfloat16, gate="highway", per_token=True),
+    dict(R=4, D=16, dtype=torch.float32, gate="highway", post=False),
+    dict(R=4, D=16, dtype=torch.float32, gate="scale", pre=False, alpha=0.7),
+]
+
+
+@pytest.mark.parametrize("case", CPU_CASES)
+def test_plain_matches_oracle(case):
+    check_case("cpu", **case)
+
+
+@pytest.mark.parametrize("norm", ["layer", "rms"])
+@pytest.mark.parametrize("gate", [None, "scale", "highway"])
+def test_plain_gradients_by_differences(norm, gate):
+    t = make(3, 6, torch.float64, "cpu", norm=norm, gate=gate, seed=2)
+    keys = [k for k in LEAVES if t[k] is not None]
+
+    def fn(*a):
+        return call({**t, **dict(zip(keys, a))}, norm, gate or "scale", 0.7)
+    assert torch.autograd.gradcheck(
+        fn, [t[k].clone().requires_grad_() for k in keys])
+
+
+def test_refusals():
+    x, w = torch.zeros(2, 3, 4), torch.ones(4)
+
+    def refused(*a, **k):
+        with pytest.raises(ValueError):
+            ops.block_norm(*a, **k)
+    refused(x, x[:1])
+    refused(x, x.bfloat16())
+    refused(x.long(), x.long())
+    refused(x[..., :0], x[..., :0])
+    refused(torch.zeros(()), torch.zeros(()))
+    refused(torch.zeros(1, 16385), torch.zeros(1, 16385))
+    refused(x, x, norm="batch")
+    refused(x, x, gate_kind="tanh")
+    refused(x, x, gate=w[:3])
+    refused(x, x, gate=torch.zeros(3, 4))
+    refused(x, x, gate=torch.zeros(2, 1, 4))
+    refused(x, x, gate=torch.zeros(2, 3, 4).bfloat16())
+    refused(x, x, post_bias=w)
+    refused(x, x, pre_scale=w[:3])
+    refused(x, x, pre_scale=w.double())
+    refused(x, x, pre_scale=w, pre_bias=w.bfloat16())
+    refused(x, x, pre_scale=w[None])
+
+
+# ------------------------------------------------------------------ on the GPU
+
+GPU_CASES = [
+    dict(R=1, D=1, dtype=torch.float32),
+    dict(R=5, D=1, dtype=torch.bfloat16, norm="rms", gate="scale"),
+    dict(R=300, D=3, dtype=torch.float32, norm="rms", gate="highway",
+         alpha=0.7),
+    dict(R=7, D=8, dtype=torch.float16),
+    dict(R=257, D=20, dtype=torch.float32, gate="scale", bias=False),
+    dict(R=33, D=64, dtype=torch.bfloat16, gate="highway", per_token=True),
+    dict(R=9, D=130, dtype=torch.float16, norm="rms", gate="scale",
+         per_token=True, alpha=0.5),
+    dict(R=1030, D=257, dtype=torch.bfloat16, gate="scale"),
+    dict(R=17, D=511, dtype=torch.float32, gate="highway"),
+    dict(R=6, D=512, dtype=torch.bfloat16, pdt=torch.float32, gate="scale"),
+    dict(R=6, D=513, dtype=torch.float16, pdt=torch.float32, gate="highway"),
+    dict(R=2500, D=1024, dtype=torch.bfloat16, gate="scale", alpha=0.5),
+    dict(R=3, D=1021, dtype=torch.float32, norm="rms"),
+    dict(R=4, D=2050, dtype=torch.bfloat16, gate="highway"),
+    dict(R=5, D=4096, dtype=torch.float32, gate="scale", per_token=True),
+    dict(R=5, D=4097, dtype=torch.bfloat16, gate="scale"),
+    dict(R=3, D=8191, dtype=torch.float32, gate="highway"),
+    dict(R=3, D=8200, dtype=torch.float16, norm="rms", gate="scale"),
+    dict(R=2, D=16384, dtype=torch.float32, gate="highway", per_token=True),
+    dict(R=9, D=96, dtype=torch.float32, post=False),
+    dict(R=9, D=96, dtype=torch.bfloat16, pre=False, gate="scale"),
+    dict(R=9, D=96, dtype=torch.bfloat16, pre=False, post=False),
+    dict(R=9, D=96, dtype=torch.float16, pre=False, post=False,
+         gate="highway", alpha=0.5),
+    dict(R=9, D=1000, dtype=torch.float32, pre=False, post=False,
+         gate="scale", per_token=True),
+    # a mean far from 0 beside the deviation
+    dict(R=12, D=700, dtype=torch.float32, shift=300.0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", GPU_CASES)
+def test_gpu_matches_oracle(case):
+    check_case("cuda", **case)
+
+
+@pytest.mark.gpu
+def test_gpu_no_rows():
+    w = torch.ones(8, device="cuda", requires_grad=True)
+    x = torch.zeros(0, 3, 8, device="cuda", requires_grad=True)
+    s, h = ops.block_norm(x, x, gate=w, post_scale=w, pre_scale=w, pre_bias=w)
+    assert s.shape == h.shape == x.shape
+    gx, gw = torch.autograd.grad((s.sum() + h.sum()), (x, w))
+    assert gx.shape == x.shape and bool((gw == 0).all())
+
+
+@pytest.mark.gpu
+def test_gpu_shapes_and_strides():
+    """Leading dimensions, views that are not dense, one row as a vector."""
+    t = make(12, 40, torch.float32, "cuda", gate="scale", per_token=True)
+    base = call(t, "layer", "scale", 1.0)
+    r = {k: v.view(3, 4, 40) if v is not None and v.dim() == 2 else v
+         for k, v in t.items()}
+    got = call(r, "layer", "scale", 1.0)
+    assert all(torch.equal(a, b.view(12, 40)) for a, b in zip(base, got))
+    wide = torch.cat([t["x"], t["res"]], 1)
+    v = {**t, "x": wide[:, :40], "res": wide[:, 40:],
+         "gate": t["gate"].t().contiguous().t(),
+         "pre_scale": t["pre_scale"].repeat_interleave(2)[::2]}
+    got = call(v, "layer", "scale", 1.0)
+    assert all(torch.equal(a, b) for a, b in zip(base, got))
+    one = {k: w[0] if w is not None and w.dim() == 2 else w
+           for k, w in t.items()}
+    got = call(one, "layer", "scale", 1.0)
+    assert all(torch.equal(a[0], b) for a, b in zip(base, got))
+
+
+@pytest.mark.gpu
+def test_gpu_partial_gradients():
+    t = make(70, 300, torch.float32, "cuda", gate="highway")
+    s, h, full = run(t, "layer", "highway", 1.0)
+    zero = torch.zeros_like(t["dsum"])
+    keys = list(full)
+    ins = [t[k] for k in keys]
+    both = call(t, "layer", "highway", 1.0)
+    for i, d in ((0, t["dsum"]), (1, t["dh"])):
+        a = torch.autograd.grad(both[i], ins, d, retain_graph=True,
+                                allow_unused=True)
+        b = torch.autograd.grad(both, ins, (d, zero) if i == 0 else (zero, d),
+                                retain_graph=True)
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+    for k in keys:      # one input at a time
+        r = {n: None if v is None else v.detach() for n, v in t.items()}
+        r[k] = r[k].clone().requires_grad_()
+        g, = torch.autograd.grad(call(r, "layer", "highway", 1.0), r[k],
+                                 (t["dsum"], t["dh"]))
+        assert torch.equal(g, full[k]), k
+
+
+@pytest.mark.gpu
+def test_gpu_bad_rows_stay_alone():
+    """NaN and infinity in one row, at the end of the last block too."""
+    for bad in (3, 44):
+        t = make(45, 100, torch.float32, "cuda", gate="scale")
+        ok = call(t, "layer", "scale", 1.0)
+        t["x"][bad, 5] = float("nan")
+        t["res"][bad, 7] = float("inf")
+        got = call(t, "layer", "scale", 1.0)
+        keep = torch.arange(45, device="cuda") != bad
+        for a, b in zip(ok, got):
+            assert torch.equal(a[keep], b[keep])
+        assert bool(torch.isnan(got[1][bad]).all())
+
+
+@pytest.mark.gpu
+def test_gpu_repeats_bit_for_bit():
+    t = make(3001, 520, torch.bfloat16, "cuda", gate="highway")
+    first = run(t, "layer", "highway", 1.0)
+    for _ in range(3):
+        again = run(t, "layer", "highway", 1.0)
+        assert torch.equal(first[0], again[0])
+        assert torch.equal(first[1], again[1])
+        assert all(torch.equal(first[2][k], again[2][k]) for k in first[2])
+
+
+@pytest.mark.gpu
+def test_gpu_captured():
+    """Forward and backward replayed from two graphs that interleave."""
+    graphs = []
+    for seed, D in ((1, 256), (2, 700)):
+        t = make(500, D, torch.bfloat16, "cuda", gate="scale", seed=seed)
+
+        def once(t=t):
+            s, h, g = run(t, "layer", "scale", 1.0)
+            return [s.detach(), h.detach()] + list(g.values())
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            once()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = once()
+        graphs.append((graph, outs, once))
+    for _ in range(3):
+        for _, outs, _ in graphs:
+            for o in outs:
+                o.zero_()
+        for graph, _, _ in graphs:
+            graph.replay()
+        for _, outs, once in graphs:
+            assert all(torch.equal(p, q) for p, q in zip(outs, once()))
