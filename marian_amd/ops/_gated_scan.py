@@ -45,8 +45,13 @@ def check_scan(what, x, gate, state, lens, act, dims):
 
 
 def dense_rows(t):
-    """t, or a copy of it if its last dimension is not dense."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    """t, or a copy of it if its last dimension is not dense or its rows lie
+    further apart than the kernels' offsets reach."""
+    if t.stride(-1) != 1 and t.shape[-1] != 1:
+        return t.contiguous()
+    if t.dim() == 3 and t.shape[1] > 1 and t.stride(1) >= 1 << 26:
+        return t.contiguous()
+    return t
 
 
 def gated_scan_torch(x, gate, state=None, lens=None, reverse=False,

@@ -18,12 +18,21 @@
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 
+#include <type_traits>
+
 #include "common.h"
 #include "vec.h"
 
 using namespace mamd;
 
+// for lambdas that work on arrays in registers
+#define ALWAYS_INLINE __attribute__((always_inline))
+
 namespace {
+
+constexpr int kLC = 32;     // lanes along the channels
+constexpr int kSteps = 8;   // steps a thread holds at a time
+constexpr int kMaxChunks = 32;
 
 struct ScanArgs {
   const void* x;
@@ -33,7 +42,10 @@ struct ScanArgs {
   const int* lens;          // [B] or null (T)
   float* bnd;               // [B,nt,D] state at each tile's start, or null
   int B, T, D;
-  int nt;                   // tiles of kTile steps
+  int ctiles;               // channel tiles of a row
+  int nt;                   // time tiles
+  int nc, tpc;              // chunks of the time axis, tiles in each
+  float* agg;               // [2][B,nc,D] the chunks' maps if nc > 1
   int reverse, relu;
   // forward
   void* y;                  // [B,T,D] contiguous
@@ -47,17 +59,171 @@ struct ScanArgs {
   float* dstate;            // [B,D] or null
 };
 
-// a tile's steps; the forward and the backward pass agree on it, since one
-// keeps the states that the other starts from
-constexpr int kTile = 64;
-
-__device__ __forceinline__ int valid_len(const ScanArgs& a, int b) {
-  return a.lens ? min(max(a.lens[b], 0), a.T) : a.T;
+// base (the same in all lanes) + a 32-bit offset per lane, kept in that form:
+// left to itself the compiler adds the two and needs a 64-bit address per row
+typedef __attribute__((address_space(1))) char gchar;
+__device__ __forceinline__ char* uniform(const void* p) {
+  const unsigned long v = (unsigned long)p;
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v);
+  const unsigned hi = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32));
+  return (char*)((unsigned long)hi << 32 | lo);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ vec_t<T, VEC> load_at(const char* base,
+                                                 unsigned lane) {
+  const gchar* q = (const gchar*)base;
+  asm("" : "+s"(q));
+  return *(const __attribute__((address_space(1)))
+               typename Vec<T, VEC>::mem*)(q + lane);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_at(char* base, unsigned lane,
+                                         const float o[VEC]) {
+  vec_t<T, VEC> r;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) r[i] = (T)o[i];
+  gchar* q = (gchar*)base;
+  asm("" : "+s"(q));
+  *(__attribute__((address_space(1))) typename Vec<T, VEC>::mem*)(q + lane) =
+      r;
 }
 
-// step s of the recurrence sits at this position of the time axis
-__device__ __forceinline__ int time_of(const ScanArgs& a, int s, int len) {
-  return a.reverse ? len - 1 - s : s;
+// Which rows, channels and steps a block works on, and where its lanes are.
+// A wave is 32 lanes of VEC channels by 2 groups of kSteps steps; the block's
+// NW waves follow each other in time. A lane whose channels would pass the
+// row's end moves back to the last VEC channels: it computes what its
+// neighbours compute and writes the same values there, so every access is
+// whole and in bounds for any D >= VEC.
+template <int VEC, int NW>
+struct Place {
+  static constexpr int kTile = 2 * NW * kSteps;
+  int b, chunk, lc, ws, wid, ch, len;
+  bool owns;
+  size_t vec0;              // this lane in a [B,D] array
+  __device__ __forceinline__ Place(const ScanArgs& a, int chunk0) {
+    const int lane = threadIdx.x & 63;
+    lc = lane & (kLC - 1), ws = lane / kLC;
+    wid = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int pair = blockIdx.x % (a.B * a.ctiles);
+    chunk = blockIdx.x / (a.B * a.ctiles) + chunk0;
+    b = pair / a.ctiles;
+    const int c = (pair % a.ctiles) * (kLC * VEC) + lc * VEC;
+    owns = c < a.D;
+    ch = min(c, a.D - VEC);
+    len = __builtin_amdgcn_readfirstlane(
+        a.lens ? min(max(a.lens[b], 0), a.T) : a.T);
+    vec0 = (size_t)b * a.D + ch;
+  }
+  // the first of this thread's steps in a tile
+  __device__ __forceinline__ int first(int tile) const {
+    return tile * kTile + (wid * 2 + ws) * kSteps;
+  }
+  // Position of step s on the time axis; padded steps (s >= len) come last.
+  __device__ __forceinline__ long time_of(const ScanArgs& a, int s) const {
+    return a.reverse && s < len ? len - 1 - s : s;
+  }
+  // A thread's rows of a tile. A wave's rows are read from a scalar base with
+  // a 32-bit lane offset (strides are below 2^26 elements), so an address
+  // costs no 64-bit arithmetic per lane and no register per row.
+  // FULL: every step exists; otherwise rows behind the sequence repeat its
+  // last one.
+  template <bool FULL, typename T>
+  __device__ __forceinline__ void load(const ScanArgs& a, const T* base,
+                                       long stride, int tile,
+                                       vec_t<T, VEC> r[kSteps]) const {
+    const int sw = tile * kTile + wid * 2 * kSteps;
+    const long bytes = stride * (long)sizeof(T);
+    if constexpr (FULL) {
+      const long d = a.reverse ? -bytes : bytes;
+      const int t0 = a.reverse ? len - 1 - kSteps - sw : sw;
+      const char* q = uniform((const char*)base + t0 * bytes);
+      const unsigned lane = (unsigned)((a.reverse ? 1 - ws : ws) * kSteps) *
+                                (unsigned)bytes +
+                            (unsigned)ch * (unsigned)sizeof(T);
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j)
+        r[j] = load_at<T, VEC>(q + j * d, lane);
+    } else {
+      const int t0 = a.reverse ? max(len - sw - 2 * kSteps, 0)
+                               : min(sw, len - 1);
+      const char* q = uniform((const char*)base + t0 * bytes);
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        const int t = time_of(a, min(sw + ws * kSteps + j, len - 1));
+        const unsigned lane = (unsigned)(t - t0) * (unsigned)bytes +
+                              (unsigned)ch * (unsigned)sizeof(T);
+        r[j] = load_at<T, VEC>(q, lane);
+      }
+    }
+  }
+  // FULL == false: up to T, padding included
+  template <bool FULL, typename T>
+  __device__ __forceinline__ void store(const ScanArgs& a, T* base,
+                                        long stride, int tile,
+                                        const float o[kSteps][VEC]) const {
+    const int sw = tile * kTile + wid * 2 * kSteps;
+    const long bytes = stride * (long)sizeof(T);
+    if constexpr (FULL) {
+      const long d = a.reverse ? -bytes : bytes;
+      const int t0 = a.reverse ? len - 1 - kSteps - sw : sw;
+      char* q = uniform((char*)base + t0 * bytes);
+      const unsigned lane = (unsigned)((a.reverse ? 1 - ws : ws) * kSteps) *
+                                (unsigned)bytes +
+                            (unsigned)ch * (unsigned)sizeof(T);
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j)
+        store_at<T, VEC>(q + j * d, lane, o[j]);
+    } else {
+      const int s0 = sw + ws * kSteps;
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j)
+        if (s0 + j < a.T)
+          store_vec<T, VEC>(base + time_of(a, s0 + j) * stride + ch, o[j]);
+    }
+  }
+};
+
+// the value of the wave's lower and of its upper half, in all lanes
+__device__ __forceinline__ void halves(float v, float& lo, float& hi) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v),
+                                                  __float_as_uint(v), false,
+                                                  false);
+  lo = __uint_as_float(r[0]);
+  hi = __uint_as_float(r[1]);
+}
+
+// From a group's map (A, H): the wave's map, and in eA, eH the map of the
+// steps of its wave that come before this group's.
+template <int VEC>
+__device__ __forceinline__ void wave_fold(int ws, float A[VEC], float H[VEC],
+                                          float eA[VEC], float eH[VEC]) {
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) {
+    float a0, a1, h0, h1;
+    halves(A[v], a0, a1);
+    halves(H[v], h0, h1);
+    A[v] = a1 * a0;
+    H[v] = a1 * h0 + h1;
+    eA[v] = ws ? a0 : 1.f;
+    eH[v] = ws ? h0 : 0.f;
+  }
+}
+
+// the same from the far end
+template <int VEC>
+__device__ __forceinline__ void wave_fold_back(int ws, float A[VEC],
+                                               float M[VEC], float eA[VEC],
+                                               float eM[VEC]) {
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) {
+    float a0, a1, m0, m1;
+    halves(A[v], a0, a1);
+    halves(M[v], m0, m1);
+    A[v] = a0 * a1;
+    M[v] = a0 * m1 + m0;
+    eA[v] = ws ? 1.f : a1;
+    eM[v] = ws ? 0.f : m1;
+  }
 }
 
 // a NaN state stays visible, which fmaxf would turn into 0
@@ -65,57 +231,103 @@ __device__ __forceinline__ float activate(float c, int relu) {
   return relu && c < 0.f ? 0.f : c;
 }
 
-// Block: LC lanes of VEC channels by SUB groups of STEPS steps. A lane whose
-// channels would pass the row's end moves back to the last VEC channels: it
-// computes what its neighbours compute and writes the same values there, so
-// every access is whole and in bounds for any D >= VEC. Steps behind the
-// sequence read position 0 and are masked.
-template <int VEC, int LC>
-__device__ __forceinline__ int lane_channel(const ScanArgs& a, int ctile,
-                                            int lc, bool& owns) {
-  const int ch = ctile * (LC * VEC) + lc * VEC;
-  owns = ch < a.D;
-  return min(ch, a.D - VEC);
+// calls fn with a compile-time truth value
+template <typename F>
+__device__ __forceinline__ void with_bool(bool v, F fn) {
+  if (v) fn(std::true_type{});
+  else fn(std::false_type{});
 }
 
-template <typename T, int VEC, int LC, int SUB>
-__global__ __launch_bounds__(LC* SUB) void scan_fwd_kernel(ScanArgs a,
-                                                           int ctiles) {
-  constexpr int STEPS = kTile / SUB;
-  __shared__ float sA[SUB][LC * VEC], sH[SUB][LC * VEC];
-  const int lc = threadIdx.x % LC, sub = threadIdx.x / LC;
-  const int b = blockIdx.x / ctiles;
-  bool owns;
-  const int ch = lane_channel<VEC, LC>(a, blockIdx.x % ctiles, lc, owns);
-  const int len = valid_len(a, b);
-  const T* x = (const T*)a.x + (size_t)b * a.xb + ch;
-  const T* g = (const T*)a.g + (size_t)b * a.gb + ch;
-  T* y = (T*)a.y + (size_t)b * a.T * a.D + ch;
-  const size_t vec0 = (size_t)b * a.D + ch;  // this lane in a [B,D] array
-
-  float c[VEC];
+// The maps of the chunks [k0, k1) from the aggregates, applied to c: every
+// wave folds some of them, one channel per lane, and the waves' maps meet in
+// LDS. back: from the last chunk to the first.
+template <int VEC, int NW>
+__device__ __forceinline__ void fold_chunks(const ScanArgs& a,
+                                            const Place<VEC, NW>& p, int k0,
+                                            int k1, bool back,
+                                            float (*sA)[kLC * VEC],
+                                            float (*sH)[kLC * VEC],
+                                            float c[VEC]) {
+  constexpr int PER = (kMaxChunks + NW - 1) / NW;
+  const int lane = threadIdx.x & 63, n = k1 - k0;
+  if (lane < kLC * VEC) {
+    const int c0 = p.b * a.ctiles;  // this block's pair, without its channels
+    const int pair = blockIdx.x % (a.B * a.ctiles) - c0;
+    const int ch = min(min(pair * (kLC * VEC) + (lane / VEC) * VEC,
+                           a.D - VEC) + lane % VEC, a.D - 1);
+    const size_t plane = (size_t)a.B * a.nc * a.D;
+    float va[PER], vh[PER];
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) c[v] = a.state ? a.state[vec0 + v] : 0.f;
-
-  for (int tile = 0; tile < a.nt; ++tile) {
-    const int s0 = tile * kTile + sub * STEPS;
-    if (a.bnd && sub == 0 && owns)
-      store_vec<float, VEC>(a.bnd + ((size_t)b * a.nt + tile) * a.D + ch, c);
-    vec_t<T, VEC> xr[STEPS], gr[STEPS];
-#pragma unroll
-    for (int j = 0; j < STEPS; ++j) {
-      const int s = s0 + j;
-      const int t = s < len ? time_of(a, s, len) : 0;
-      xr[j] = load_vec<T, VEC>(x + (size_t)t * a.xt);
-      gr[j] = load_vec<T, VEC>(g + (size_t)t * a.gt);
+    for (int i = 0; i < PER; ++i) {  // r-th map to apply; past n: the last
+      const int r = min(p.wid * PER + i, n - 1);
+      const float* q =
+          a.agg + ((size_t)p.b * a.nc + (back ? k1 - 1 - r : k0 + r)) * a.D +
+          ch;
+      va[i] = q[0];
+      vh[i] = q[plane];
     }
-    float f[STEPS][VEC], h[STEPS][VEC];
-    float A[VEC], H[VEC];
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (p.wid * PER + i >= n) va[i] = 1.f, vh[i] = 0.f;
+    float A = 1.f, H = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) H = va[i] * H + vh[i], A *= va[i];
+    sA[p.wid][lane] = A;
+    sH[p.wid][lane] = H;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < NW; ++w)
+#pragma unroll
+    for (int v = 0; v < VEC; ++v)
+      c[v] = sA[w][p.lc * VEC + v] * c[v] + sH[w][p.lc * VEC + v];
+  __syncthreads();
+}
+
+// AGG: only the chunk's map, for the blocks of the pass that follows.
+template <typename T, int VEC, int NW, bool AGG>
+__global__ __launch_bounds__(NW * 64) void scan_fwd_kernel(ScanArgs a) {
+  __shared__ float sA[2][NW][kLC * VEC], sH[2][NW][kLC * VEC];
+  using P = Place<VEC, NW>;
+  const P p(a, 0);
+  const T* x = (const T*)a.x + (size_t)p.b * a.xb;
+  const T* g = (const T*)a.g + (size_t)p.b * a.gb;
+  T* y = (T*)a.y + (size_t)p.b * a.T * a.D;
+  const int k0 = p.chunk * a.tpc, k1 = min(k0 + a.tpc, a.nt);
+  // tiles full of steps, and tiles with a step; what follows is padding
+  const int kf = min(k1, p.len / P::kTile);
+  const int kv = min(k1, (p.len + P::kTile - 1) / P::kTile);
+
+  vec_t<T, VEC> xr[kSteps], gr[kSteps];
+  auto fetch = [&](int tile, auto full) ALWAYS_INLINE {
+    constexpr bool FULL = decltype(full)::value;
+    p.template load<FULL>(a, x, a.xt, tile, xr);
+    p.template load<FULL>(a, g, a.gt, tile, gr);
+  };
+  if (k0 < kf) fetch(k0, std::true_type{});
+
+  float c[VEC], Ap[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) {
+    c[v] = !AGG && a.state ? a.state[p.vec0 + v] : 0.f;
+    Ap[v] = 1.f;
+  }
+  if (!AGG && p.chunk > 0)
+    fold_chunks<VEC, NW>(a, p, 0, p.chunk, false, sA[0], sH[0], c);
+
+  auto body = [&](int tile, auto full) ALWAYS_INLINE {
+    constexpr bool FULL = decltype(full)::value;
+    const int s0 = p.first(tile), buf = tile & 1;
+    if (!AGG && a.bnd && threadIdx.x < kLC && p.owns)
+      store_vec<float, VEC>(a.bnd + ((size_t)p.b * a.nt + tile) * a.D + p.ch,
+                            c);
+    float f[kSteps][VEC], h[kSteps][VEC];
+    float A[VEC], H[VEC], eA[VEC], eH[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) A[v] = 1.f, H[v] = 0.f;
 #pragma unroll
-    for (int j = 0; j < STEPS; ++j) {
-      const bool on = s0 + j < len;
+    for (int j = 0; j < kSteps; ++j) {
+      const bool on = FULL || s0 + j < p.len;
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
         float ff, om;
@@ -126,87 +338,147 @@ __global__ __launch_bounds__(LC* SUB) void scan_fwd_kernel(ScanArgs a,
         H[v] = f[j][v] * H[v] + h[j][v];
       }
     }
+    if (FULL && tile + 1 < kf) fetch(tile + 1, full);
+    wave_fold<VEC>(p.ws, A, H, eA, eH);
+    if (p.ws == 0) {
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      sA[sub][lc * VEC + v] = A[v];
-      sH[sub][lc * VEC + v] = H[v];
+      for (int v = 0; v < VEC; ++v) {
+        sA[buf][p.wid][p.lc * VEC + v] = A[v];
+        sH[buf][p.wid][p.lc * VEC + v] = H[v];
+      }
     }
     __syncthreads();
     float cur[VEC];
 #pragma unroll
-    for (int k = 0; k < SUB; ++k) {
+    for (int w = 0; w < NW; ++w)
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
-        if (k == sub) cur[v] = c[v];
-        c[v] = sA[k][lc * VEC + v] * c[v] + sH[k][lc * VEC + v];
+        if (w == p.wid) cur[v] = c[v];
+        const float wa = sA[buf][w][p.lc * VEC + v];
+        c[v] = wa * c[v] + sH[buf][w][p.lc * VEC + v];
+        if constexpr (AGG) Ap[v] *= wa;
       }
-    }
-    __syncthreads();
-    if (owns) {
+    if constexpr (!AGG) {
 #pragma unroll
-      for (int j = 0; j < STEPS; ++j) {
-        const int s = s0 + j;
-        float o[VEC];
+      for (int v = 0; v < VEC; ++v) cur[v] = eA[v] * cur[v] + eH[v];
+      with_bool(a.relu, [&](auto relu) ALWAYS_INLINE {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          cur[v] = f[j][v] * cur[v] + h[j][v];
-          o[v] = s < len ? activate(cur[v], a.relu) : 0.f;
-        }
-        if (s < a.T)
-          store_vec<T, VEC>(
-              y + (size_t)(s < len ? time_of(a, s, len) : s) * a.D, o);
+        for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) {
+            cur[v] = f[j][v] * cur[v] + h[j][v];
+            h[j][v] = activate(cur[v], decltype(relu)::value);
+          }
+      });
+      if constexpr (!FULL) {
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+          for (int v = 0; v < VEC; ++v)
+            if (s0 + j >= p.len) h[j][v] = 0.f;
       }
+      if (p.owns) p.template store<FULL>(a, y, (long)a.D, tile, h);
     }
+  };
+  for (int tile = k0; tile < kf; ++tile) body(tile, std::true_type{});
+  if (k0 < kv && kf < kv) {
+    fetch(kv - 1, std::false_type{});
+    body(kv - 1, std::false_type{});
   }
-  if (sub == 0 && owns) store_vec<float, VEC>(a.last + vec0, c);
+  if constexpr (AGG) {
+    if (threadIdx.x < kLC && p.owns) {
+      float* q = a.agg + ((size_t)p.b * a.nc + p.chunk) * a.D + p.ch;
+      store_vec<float, VEC>(q, Ap);
+      store_vec<float, VEC>(q + (size_t)a.B * a.nc * a.D, c);
+    }
+  } else {
+    const float zero[VEC] = {};
+    for (int tile = max(kv, k0); tile < k1; ++tile) {
+      if (a.bnd && threadIdx.x < kLC && p.owns)
+        store_vec<float, VEC>(
+            a.bnd + ((size_t)p.b * a.nt + tile) * a.D + p.ch, c);
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        const int s = p.first(tile) + j;
+        if (s < a.T && p.owns) store_vec<T, VEC>(y + (size_t)s * a.D + p.ch, zero);
+      }
+    }
+    if (p.chunk == a.nc - 1 && threadIdx.x < kLC && p.owns)
+      store_vec<float, VEC>(a.last + p.vec0, c);
+  }
 }
 
-template <typename T, int VEC, int LC, int SUB>
-__global__ __launch_bounds__(LC* SUB) void scan_bwd_kernel(ScanArgs a,
-                                                           int ctiles) {
-  constexpr int STEPS = kTile / SUB;
-  __shared__ float sA[SUB][LC * VEC], sH[SUB][LC * VEC], sM[SUB][LC * VEC];
-  const int lc = threadIdx.x % LC, sub = threadIdx.x / LC;
-  const int b = blockIdx.x / ctiles;
-  bool owns;
-  const int ch = lane_channel<VEC, LC>(a, blockIdx.x % ctiles, lc, owns);
-  const int len = valid_len(a, b);
-  const T* x = (const T*)a.x + (size_t)b * a.xb + ch;
-  const T* g = (const T*)a.g + (size_t)b * a.gb + ch;
-  const T* dy = a.dy ? (const T*)a.dy + (size_t)b * a.T * a.D + ch : nullptr;
-  T* dx = (T*)a.dx + (size_t)b * a.dxb + ch;
-  T* dg = (T*)a.dg + (size_t)b * a.dgb + ch;
-  const size_t vec0 = (size_t)b * a.D + ch;
+// AGG: only the chunk's map of mu.
+template <typename T, int VEC, int NW, bool AGG>
+__global__ __launch_bounds__(NW * 64) void scan_bwd_kernel(ScanArgs a) {
+  __shared__ float sA[2][NW][kLC * VEC], sH[2][NW][kLC * VEC];
+  __shared__ float sM[2][NW][kLC * VEC];
+  using P = Place<VEC, NW>;
+  const P p(a, AGG ? 1 : 0);
+  const T* x = (const T*)a.x + (size_t)p.b * a.xb;
+  const T* g = (const T*)a.g + (size_t)p.b * a.gb;
+  const T* dy =
+      a.dy ? (const T*)a.dy + (size_t)p.b * a.T * a.D : nullptr;
+  T* dx = (T*)a.dx + (size_t)p.b * a.dxb;
+  T* dg = (T*)a.dg + (size_t)p.b * a.dgb;
+  const int k0 = p.chunk * a.tpc, k1 = min(k0 + a.tpc, a.nt);
+  const int kf = min(k1, p.len / P::kTile);
+  const int kv = min(k1, (p.len + P::kTile - 1) / P::kTile);
+  // the map of mu needs the states for relu's side only
+  const bool states = !AGG || a.relu;
 
-  float mu[VEC];
+  vec_t<T, VEC> xr[kSteps], gr[kSteps], dr[kSteps];
+  float cr[VEC];            // the state at the tile's start
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) mu[v] = a.dlast ? a.dlast[vec0 + v] : 0.f;
+  for (int j = 0; j < kSteps; ++j) xr[j] = dr[j] = {};
+  auto fetch = [&](int tile, auto full) ALWAYS_INLINE {
+    constexpr bool FULL = decltype(full)::value;
+    if (states) p.template load<FULL>(a, x, a.xt, tile, xr);
+    p.template load<FULL>(a, g, a.gt, tile, gr);
+    if (dy) p.template load<FULL>(a, dy, (long)a.D, tile, dr);
+    const float* cp =
+        a.bnd ? a.bnd + ((size_t)p.b * a.nt + tile) * a.D + p.ch
+              : (a.state ? a.state + p.vec0 : nullptr);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) cr[v] = cp && states ? cp[v] : 0.f;
+  };
+  const bool rest = k0 < kv && kf < kv;  // the last of them is not full
+  if (rest)
+    fetch(kv - 1, std::false_type{});
+  else if (k0 < kf)
+    fetch(kf - 1, std::true_type{});
 
-  for (int tile = a.nt - 1; tile >= 0; --tile) {
-    const int s0 = tile * kTile + sub * STEPS;
-    vec_t<T, VEC> xr[STEPS], gr[STEPS], dr[STEPS];
+  float mu[VEC], Ap[VEC];
 #pragma unroll
-    for (int j = 0; j < STEPS; ++j) {
-      const int s = s0 + j;
-      const int t = s < len ? time_of(a, s, len) : 0;
-      xr[j] = load_vec<T, VEC>(x + (size_t)t * a.xt);
-      gr[j] = load_vec<T, VEC>(g + (size_t)t * a.gt);
-      dr[j] = {};
-      if (dy) dr[j] = load_vec<T, VEC>(dy + (size_t)t * a.D);
-    }
-    // the state at this tile's start
-    const float* cp = a.bnd ? a.bnd + ((size_t)b * a.nt + tile) * a.D + ch
-                            : (a.state ? a.state + vec0 : nullptr);
-    float A[VEC], H[VEC], c[VEC];
+  for (int v = 0; v < VEC; ++v) {
+    mu[v] = !AGG && a.dlast ? a.dlast[p.vec0 + v] : 0.f;
+    Ap[v] = 1.f;
+  }
+  if (!AGG && p.chunk < a.nc - 1)
+    fold_chunks<VEC, NW>(a, p, p.chunk + 1, a.nc, true, sA[0], sH[0], mu);
+
+  if constexpr (!AGG) {
+    const float zero[VEC] = {};
+    for (int tile = max(kv, k0); tile < k1; ++tile)
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      A[v] = 1.f, H[v] = 0.f;
-      c[v] = cp ? cp[v] : 0.f;
-    }
-    float f[STEPS][VEC], om[STEPS][VEC], w[STEPS][VEC], d[STEPS][VEC];
+      for (int j = 0; j < kSteps; ++j) {
+        const int s = p.first(tile) + j;
+        if (s < a.T && p.owns) {
+          store_vec<T, VEC>(dx + (size_t)s * a.dxt + p.ch, zero);
+          store_vec<T, VEC>(dg + (size_t)s * a.dgt + p.ch, zero);
+        }
+      }
+  }
+  auto body = [&](int tile, auto full) ALWAYS_INLINE {
+    constexpr bool FULL = decltype(full)::value;
+    const int s0 = p.first(tile), buf = tile & 1;
+    float f[kSteps][VEC], om[kSteps][VEC], w[kSteps][VEC], d[kSteps][VEC];
+    float A[VEC], H[VEC], A2[VEC], eA[VEC], eH[VEC], c[VEC];
 #pragma unroll
-    for (int j = 0; j < STEPS; ++j) {
-      const bool on = s0 + j < len;
+    for (int v = 0; v < VEC; ++v) A[v] = 1.f, H[v] = 0.f, c[v] = cr[v];
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      const bool on = FULL || s0 + j < p.len;
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
         float ff, oo;
@@ -219,69 +491,99 @@ __global__ __launch_bounds__(LC* SUB) void scan_bwd_kernel(ScanArgs a,
         H[v] = f[j][v] * H[v] + om[j][v] * w[j][v];
       }
     }
+    if (tile > k0) fetch(tile - 1, std::true_type{});
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      sA[sub][lc * VEC + v] = A[v];
-      sH[sub][lc * VEC + v] = H[v];
-    }
-    __syncthreads();
+    for (int v = 0; v < VEC; ++v) A2[v] = A[v];
+    if (states) {
+      wave_fold<VEC>(p.ws, A, H, eA, eH);
+      if (p.ws == 0) {
 #pragma unroll
-    for (int k = 0; k < SUB - 1; ++k)
-#pragma unroll
-      for (int v = 0; v < VEC; ++v)
-        if (k < sub) c[v] = sA[k][lc * VEC + v] * c[v] + sH[k][lc * VEC + v];
-    // w becomes c_{t-1} - x_t, d is cut where relu was off
-#pragma unroll
-    for (int j = 0; j < STEPS; ++j)
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        const float xv = w[j][v];
-        w[j][v] = c[v] - xv;
-        c[v] = f[j][v] * c[v] + om[j][v] * xv;
-        if (a.relu && c[v] <= 0.f) d[j][v] = 0.f;
+        for (int v = 0; v < VEC; ++v) {
+          sA[buf][p.wid][p.lc * VEC + v] = A[v];
+          sH[buf][p.wid][p.lc * VEC + v] = H[v];
+        }
       }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < NW - 1; ++k)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v)
+          if (k < p.wid)
+            c[v] = sA[buf][k][p.lc * VEC + v] * c[v] +
+                   sH[buf][k][p.lc * VEC + v];
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) c[v] = eA[v] * c[v] + eH[v];
+      // w becomes c_{t-1} - x_t, d is cut where relu was off
+      with_bool(a.relu, [&](auto relu) ALWAYS_INLINE {
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) {
+            const float xv = w[j][v];
+            w[j][v] = c[v] - xv;
+            c[v] = f[j][v] * c[v] + om[j][v] * xv;
+            if (decltype(relu)::value && c[v] <= 0.f) d[j][v] = 0.f;
+          }
+      });
+    }
     // this thread's steps from the far end, with nothing coming in
-    float M[VEC];
+    float M[VEC], eM[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) M[v] = 0.f;
 #pragma unroll
-    for (int j = STEPS - 1; j >= 0; --j)
+    for (int j = kSteps - 1; j >= 0; --j)
 #pragma unroll
       for (int v = 0; v < VEC; ++v) M[v] = f[j][v] * (d[j][v] + M[v]);
+    wave_fold_back<VEC>(p.ws, A2, M, eA, eM);
+    if (p.ws == 0) {
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) sM[sub][lc * VEC + v] = M[v];
+      for (int v = 0; v < VEC; ++v) {
+        sM[buf][p.wid][p.lc * VEC + v] = M[v];
+        if (!states) sA[buf][p.wid][p.lc * VEC + v] = A2[v];
+      }
+    }
     __syncthreads();
     float cur[VEC];
 #pragma unroll
-    for (int k = SUB - 1; k >= 0; --k)
+    for (int k = NW - 1; k >= 0; --k)
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
-        if (k == sub) cur[v] = mu[v];
-        mu[v] = sA[k][lc * VEC + v] * mu[v] + sM[k][lc * VEC + v];
+        if (k == p.wid) cur[v] = mu[v];
+        const float wa = sA[buf][k][p.lc * VEC + v];
+        mu[v] = wa * mu[v] + sM[buf][k][p.lc * VEC + v];
+        if constexpr (AGG) Ap[v] *= wa;
       }
-    __syncthreads();
-    if (owns) {
+    if constexpr (!AGG) {
 #pragma unroll
-      for (int j = STEPS - 1; j >= 0; --j) {
-        const int s = s0 + j;
-        float ox[VEC], og[VEC];
+      for (int v = 0; v < VEC; ++v) cur[v] = eA[v] * cur[v] + eM[v];
+#pragma unroll
+      for (int j = kSteps - 1; j >= 0; --j) {
+        const bool on = FULL || s0 + j < p.len;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
           const float lam = d[j][v] + cur[v];
           cur[v] = f[j][v] * lam;
-          ox[v] = s < len ? om[j][v] * lam : 0.f;
-          og[v] = s < len ? cur[v] * om[j][v] * w[j][v] : 0.f;
-        }
-        if (s < a.T) {
-          const int t = s < len ? time_of(a, s, len) : s;
-          store_vec<T, VEC>(dx + (size_t)t * a.dxt, ox);
-          store_vec<T, VEC>(dg + (size_t)t * a.dgt, og);
+          d[j][v] = on ? om[j][v] * lam : 0.f;
+          w[j][v] = on ? cur[v] * om[j][v] * w[j][v] : 0.f;
         }
       }
+      if (p.owns) {
+        p.template store<FULL>(a, dx, a.dxt, tile, d);
+        p.template store<FULL>(a, dg, a.dgt, tile, w);
+      }
     }
+  };
+  if (rest) body(kv - 1, std::false_type{});
+  for (int tile = kf - 1; tile >= k0; --tile) body(tile, std::true_type{});
+  if constexpr (AGG) {
+    if (threadIdx.x < kLC && p.owns) {
+      float* q = a.agg + ((size_t)p.b * a.nc + p.chunk) * a.D + p.ch;
+      store_vec<float, VEC>(q, Ap);
+      store_vec<float, VEC>(q + (size_t)a.B * a.nc * a.D, mu);
+    }
+  } else if (a.dstate && p.chunk == 0 && threadIdx.x < kLC && p.owns) {
+    store_vec<float, VEC>(a.dstate + p.vec0, mu);
   }
-  if (a.dstate && sub == 0 && owns)
-    store_vec<float, VEC>(a.dstate + vec0, mu);
 }
 
 // one token for each row: the recurrence at T = 1, on a pool of states.
@@ -363,6 +665,17 @@ const int* lens_ptr(const c10::optional<torch::Tensor>& l,
   return l->data_ptr<int>();
 }
 
+int waves_of(int T) { return T <= 16 ? 1 : 4; }
+int vec_of_width(int D) { return D >= 2 ? 2 : 1; }
+
+// the kernels' lane offsets are 32 bits over 16 rows
+long time_stride(const torch::Tensor& t) {
+  if (t.size(1) <= 1) return 0;
+  TORCH_CHECK(t.stride(1) < (1L << 26),
+              "gated_scan: time strides must stay below 2^26 elements");
+  return t.stride(1);
+}
+
 ScanArgs base_args(const torch::Tensor& x, const torch::Tensor& g,
                    const c10::optional<torch::Tensor>& state,
                    const c10::optional<torch::Tensor>& lens, bool reverse,
@@ -370,17 +683,30 @@ ScanArgs base_args(const torch::Tensor& x, const torch::Tensor& g,
   check_rows(x, g, "gated_scan");
   TORCH_CHECK(x.dim() == 3, "gated_scan: x must be [B, T, D]");
   TORCH_CHECK(x.size(0) < (1 << 30) && x.size(1) < (1 << 30) &&
-                  x.size(2) < (1 << 30),
-              "gated_scan: sizes must stay below 2^30");
+                  x.size(2) < (1 << 26),
+              "gated_scan: B and T must stay below 2^30, D below 2^26");
   ScanArgs a{};
   a.x = x.data_ptr();
   a.g = g.data_ptr();
-  a.xb = x.stride(0), a.xt = x.stride(1);
-  a.gb = g.stride(0), a.gt = g.stride(1);
+  a.xb = x.stride(0), a.xt = time_stride(x);
+  a.gb = g.stride(0), a.gt = time_stride(g);
   a.state = state_ptr(state, x, "state");
   a.lens = lens_ptr(lens, x);
   a.B = x.size(0), a.T = x.size(1), a.D = x.size(2);
-  a.nt = (a.T + kTile - 1) / kTile;
+  // a tile holds 16 steps per wave; short sequences take fewer waves. The
+  // forward and the backward pass get the same tiles, since one keeps the
+  // states that the other starts from.
+  const int tile = 16 * waves_of(a.T);
+  a.ctiles = (a.D + vec_of_width(a.D) * kLC - 1) / (vec_of_width(a.D) * kLC);
+  a.nt = (a.T + tile - 1) / tile;
+  const long pairs = (long)a.B * a.ctiles;
+  const int nc = pairs >= 192 || pairs == 0
+                     ? 1
+                     : (int)std::min<long>({kMaxChunks, (long)a.nt,
+                                            (512 + pairs - 1) / pairs});
+  a.tpc = nc > 1 ? (a.nt + nc - 1) / nc : std::max(a.nt, 1);
+  a.nc = std::max((a.nt + a.tpc - 1) / a.tpc, 1);
+  TORCH_CHECK(pairs < (1L << 31), "gated_scan: too many rows");
   a.reverse = reverse;
   a.relu = act_code(act);
   return a;
@@ -392,10 +718,43 @@ ScanArgs base_args(const torch::Tensor& x, const torch::Tensor& g,
   else if (st == torch::kFloat32) { FN(float); }                    \
   else TORCH_CHECK(false, "gated_scan: unsupported dtype");
 
-int grid_of(const ScanArgs& a, int ctiles) {
-  const long n = (long)a.B * ctiles;
-  TORCH_CHECK(n < (1L << 31), "gated_scan: too many rows");
-  return (int)n;
+template <bool AGG>
+void launch(bool bwd, const torch::Tensor& x, const ScanArgs& a,
+            hipStream_t stream) {
+  // no chunk follows the last one (backward: the first): its map is not used
+  const long blocks = (long)a.B * a.ctiles * (AGG ? a.nc - 1 : a.nc);
+  const int nw = waves_of(a.T);
+  TORCH_CHECK(blocks * nw * 64 < (1L << 32), "gated_scan: too many rows");
+  const dim3 grid((unsigned)blocks);
+#define RUN2(ET, VEC, NW)                                                    \
+  if (bwd)                                                                   \
+    hipLaunchKernelGGL((scan_bwd_kernel<ET, VEC, NW, AGG>), grid,            \
+                       dim3(NW * 64), 0, stream, a);                         \
+  else                                                                       \
+    hipLaunchKernelGGL((scan_fwd_kernel<ET, VEC, NW, AGG>), grid,            \
+                       dim3(NW * 64), 0, stream, a)
+#define RUN1(ET, VEC)                                                        \
+  if (nw == 1) { RUN2(ET, VEC, 1); }                                         \
+  else { RUN2(ET, VEC, 4); }
+#define RUN(ET)                                                              \
+  if (vec_of_width(a.D) == 2) { RUN1(ET, 2) } else { RUN1(ET, 1) }
+  SCAN_DTYPES(x.scalar_type(), RUN)
+#undef RUN
+#undef RUN1
+#undef RUN2
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+}
+
+void run(bool bwd, const torch::Tensor& x, ScanArgs& a) {
+  auto stream = at::cuda::getCurrentHIPStream();
+  torch::Tensor agg;
+  if (a.nc > 1) {
+    agg = torch::empty({2, a.B, a.nc, a.D},
+                       x.options().dtype(torch::kFloat32));
+    a.agg = agg.data_ptr<float>();
+    launch<true>(bwd, x, a, stream);
+  }
+  launch<false>(bwd, x, a, stream);
 }
 
 }  // namespace
@@ -419,18 +778,7 @@ std::vector<torch::Tensor> gated_scan_fwd(torch::Tensor x, torch::Tensor gate,
   a.y = y.data_ptr();
   a.last = last.data_ptr<float>();
   if (a.B == 0) return {y, last, bnd};
-  auto stream = at::cuda::getCurrentHIPStream();
-#define LAUNCH(T, VEC)                                                       \
-  const int ctiles = (a.D + 64 * VEC - 1) / (64 * VEC);                      \
-  hipLaunchKernelGGL((scan_fwd_kernel<T, VEC, 64, 4>),                       \
-                     dim3(grid_of(a, ctiles)), dim3(256), 0, stream, a,      \
-                     ctiles)
-#define RUN(T)                                                               \
-  if (a.D >= 4) { LAUNCH(T, 4); } else { LAUNCH(T, 1); }
-  SCAN_DTYPES(x.scalar_type(), RUN)
-#undef RUN
-#undef LAUNCH
-  C10_HIP_KERNEL_LAUNCH_CHECK();
+  run(false, x, a);
   return {y, last, bnd};
 }
 
@@ -470,25 +818,14 @@ torch::Tensor gated_scan_bwd(torch::Tensor x, torch::Tensor gate,
   a.dlast = state_ptr(dlast, x, "dlast");
   a.dx = dx.data_ptr();
   a.dg = dgate.data_ptr();
-  a.dxb = dx.stride(0), a.dxt = dx.stride(1);
-  a.dgb = dgate.stride(0), a.dgt = dgate.stride(1);
+  a.dxb = dx.stride(0), a.dxt = time_stride(dx);
+  a.dgb = dgate.stride(0), a.dgt = time_stride(dgate);
   auto f32 = x.options().dtype(torch::kFloat32);
   auto dstate = want_dstate ? torch::empty({a.B, a.D}, f32)
                             : torch::empty({0}, f32);
   if (want_dstate) a.dstate = dstate.data_ptr<float>();
   if (a.B == 0) return dstate;
-  auto stream = at::cuda::getCurrentHIPStream();
-#define LAUNCH(T, VEC)                                                       \
-  const int ctiles = (a.D + 64 * VEC - 1) / (64 * VEC);                      \
-  hipLaunchKernelGGL((scan_bwd_kernel<T, VEC, 64, 4>),                       \
-                     dim3(grid_of(a, ctiles)), dim3(256), 0, stream, a,      \
-                     ctiles)
-#define RUN(T)                                                               \
-  if (a.D >= 2) { LAUNCH(T, 2); } else { LAUNCH(T, 1); }
-  SCAN_DTYPES(x.scalar_type(), RUN)
-#undef RUN
-#undef LAUNCH
-  C10_HIP_KERNEL_LAUNCH_CHECK();
+  run(true, x, a);
   return dstate;
 }
 
@@ -510,7 +847,7 @@ torch::Tensor gated_step(torch::Tensor x, torch::Tensor gate,
   const int vpr = (int)((D + 3) / 4);
   const long n_vec = N * vpr;
   const long grid = (n_vec + 255) / 256;
-  TORCH_CHECK(grid < (1L << 31), "gated_step: too many rows");
+  TORCH_CHECK(grid * 256 < (1L << 32), "gated_step: too many rows");
 #define RUN(T)                                                               \
   hipLaunchKernelGGL((step_kernel<T, 4>), dim3((unsigned)grid), dim3(256),   \
                      0, stream, (const T*)x.data_ptr(),                      \

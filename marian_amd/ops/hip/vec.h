@@ -35,16 +35,26 @@ __device__ __forceinline__ void store_vec(T* p, const float o[VEC]) {
 
 // f = sigmoid(g) and om = 1 - f, each to its own relative precision: with
 // e = exp(-|g|) they are 1/(1+e) and e/(1+e), neither of which cancels.
-// 16-bit inputs take the hardware's exp2 and reciprocal (about 1 ulp of 32
-// bits each, 2^-14 of a bf16 step); 32-bit inputs take the library's.
+// e is the hardware's exp2 of t = -|g| log2(e). 16-bit inputs take it and the
+// hardware's reciprocal as they are: t's rounding is worth |g| units of 32
+// bits, 2^-12 of a bf16 step at |g| = 16. 32-bit inputs add what t's rounding
+// left out, and one Newton step to the reciprocal: about 2 units, in half the
+// instructions of a library exp and divide (1.4 times the scan's speed).
 template <typename T>
 __device__ __forceinline__ void sigmoid2(float g, float& f, float& om) {
-  float e, r;
+  constexpr float kL2 = 1.44269504f, kL2Lo = 1.92596299e-8f;  // log2(e)
+  float a = fabsf(g), e, r;
   if constexpr (sizeof(T) == 4) {
-    e = expf(-fabsf(g));
-    r = 1.f / (1.f + e);
+    a = a > 200.f ? 200.f : a;  // e is 0 from there on; NaN stays
+    const float t = a * kL2;
+    const float lo = fmaf(a, kL2Lo, fmaf(a, kL2, -t));
+    e = __builtin_amdgcn_exp2f(-t);
+    e = fmaf(e * lo, -0.693147181f, e);
+    const float d = 1.f + e;
+    r = __builtin_amdgcn_rcpf(d);
+    r = fmaf(fmaf(-d, r, 1.f), r, r);
   } else {
-    e = __builtin_amdgcn_exp2f(-1.4426950408889634f * fabsf(g));
+    e = __builtin_amdgcn_exp2f(-kL2 * a);
     r = __builtin_amdgcn_rcpf(1.f + e);
   }
   const float s = e * r;

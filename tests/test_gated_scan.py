@@ -236,6 +236,14 @@ GPU_CASES = [
     dict(B=1, T=1025, D=256, dtype=torch.bfloat16, layout="fused"),
     dict(B=2, T=40, D=6, dtype=torch.float32, act="relu", lens="ragged"),
     dict(B=2, T=40, D=6, dtype=torch.float32, act="relu", reverse=True),
+    # the time axis split over blocks, with relu, raggedness and both ways
+    dict(B=1, T=150, D=2, dtype=torch.float32, act="relu"),
+    dict(B=2, T=140, D=2, dtype=torch.float32, act="relu", lens="ragged",
+         reverse=True),
+    dict(B=7, T=700, D=40, dtype=torch.float32, lens="ragged"),
+    dict(B=7, T=700, D=41, dtype=torch.bfloat16, lens="ragged", reverse=True,
+         layout="views"),
+    dict(B=1, T=4200, D=1, dtype=torch.float16),
     dict(B=300, T=3, D=17, dtype=torch.float16, lens="ragged"),
 ]
 
