@@ -265,26 +265,16 @@ def block_norm(x: torch.Tensor, res: torch.Tensor,
     from the 32-bit s; s and h are rounded once. Differentiable once in every
     tensor.
     """
-    from ._block_norm import BlockNormFn, block_norm_torch, check_join
+    if _on_gpu(x):
+        return hip_ext(required=True).block_norm(
+            x, res, gate, gate_kind, res_scale, post_scale, post_bias,
+            pre_scale, pre_bias, norm, eps)
+    from ._block_norm import block_norm_torch, check_join
     check_join(x, res, gate, gate_kind,
                {"post_scale": post_scale, "post_bias": post_bias,
                 "pre_scale": pre_scale, "pre_bias": pre_bias}, norm)
-    if not _on_gpu(x):
-        return block_norm_torch(x, res, gate, gate_kind, res_scale,
-                                post_scale, post_bias, pre_scale, pre_bias,
-                                norm, eps)
-    D = x.shape[-1]
-    if gate is not None and (gate.dim() > 1 or x.dim() == 1):
-        gate = gate.reshape(-1, D).contiguous()
-    vec = [None if v is None else v.contiguous()
-           for v in (post_scale, post_bias, pre_scale, pre_bias)]
-    if gate is not None and gate.dim() == 1:
-        gate = gate.contiguous()
-    s, h = BlockNormFn.apply(
-        x.reshape(-1, D).contiguous(), res.reshape(-1, D).contiguous(), gate,
-        *vec, gate_kind == "highway", float(res_scale), norm == "rms",
-        float(eps))
-    return s.view(x.shape), h.view(x.shape) if pre_scale is not None else None
+    return block_norm_torch(x, res, gate, gate_kind, res_scale, post_scale,
+                            post_bias, pre_scale, pre_bias, norm, eps)
 
 
 # ---------------------------------------------------------------------------
@@ -310,14 +300,11 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor,
     step (`state` itself for a row of no steps). States are held in 32 bits.
     Differentiable once in x, gate and state.
     """
-    from ._gated_scan import (GatedScanFn, check_scan, dense_rows,
-                              gated_scan_torch)
-    check_scan("gated_scan", x, gate, state, lens, act, 3)
     if _on_gpu(x):
-        return GatedScanFn.apply(
-            dense_rows(x), dense_rows(gate),
-            None if state is None else state.contiguous(),
-            None if lens is None else lens.contiguous(), bool(reverse), act)
+        return hip_ext(required=True).gated_scan(x, gate, state, lens,
+                                                 reverse, act)
+    from ._gated_scan import check_scan, gated_scan_torch
+    check_scan("gated_scan", x, gate, state, lens, act, 3)
     return gated_scan_torch(x, gate, state, lens, reverse, act)
 
 
@@ -326,19 +313,17 @@ def gated_scan_xg(xg: torch.Tensor, state: Optional[torch.Tensor] = None,
                   act: str = "none"):
     """gated_scan on a fused projection xg [B, T, 2D], values first, gates
     second: read in place, and one gradient buffer comes out."""
-    from ._gated_scan import (GatedScanXGFn, check_scan, dense_rows,
-                              gated_scan_torch)
+    if _on_gpu(xg):
+        return hip_ext(required=True).gated_scan_xg(xg, state, lens, reverse,
+                                                    act)
+    from ._gated_scan import check_scan, gated_scan_torch
     if xg.dim() != 3 or xg.shape[-1] % 2:
         raise ValueError("gated_scan_xg: xg must be [B, T, 2D], got "
                          f"{tuple(xg.shape)}")
     d = xg.shape[-1] // 2
-    check_scan("gated_scan_xg", xg[..., :d], xg[..., d:], state, lens, act, 3)
-    if _on_gpu(xg):
-        return GatedScanXGFn.apply(
-            dense_rows(xg), None if state is None else state.contiguous(),
-            None if lens is None else lens.contiguous(), bool(reverse), act)
-    return gated_scan_torch(xg[..., :d], xg[..., d:], state, lens, reverse,
-                            act)
+    x, gate = xg[..., :d], xg[..., d:]
+    check_scan("gated_scan_xg", x, gate, state, lens, act, 3)
+    return gated_scan_torch(x, gate, state, lens, reverse, act)
 
 
 def gated_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor,
@@ -350,26 +335,18 @@ def gated_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor,
     as a captured decode step needs; that call has no gradient. Otherwise a
     call that needs gradients runs as gated_scan over one position.
     """
-    from ._gated_scan import check_scan, dense_rows, gated_scan_torch
+    if _on_gpu(x):
+        return hip_ext(required=True).gated_step(x, gate, state, act, inplace)
+    from ._gated_scan import check_scan, gated_scan_torch
     if state is None:
         raise ValueError("gated_step: state is required")
     check_scan("gated_step", x, gate, state, None, act, 2)
-    grad = torch.is_grad_enabled() and (
-        x.requires_grad or gate.requires_grad or state.requires_grad)
     if inplace:
-        if grad:
+        if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad
+                                        or state.requires_grad):
             raise ValueError("gated_step: inplace has no gradient")
         if not state.is_contiguous():
             raise ValueError("gated_step: inplace needs a dense state")
-    elif grad:
-        y, new = gated_scan(x[:, None], gate[:, None], state, act=act)
-        return y[:, 0], new
-    if _on_gpu(x):
-        state = state.contiguous()
-        out = state if inplace else torch.empty_like(state)
-        y = hip_ext(required=True).gated_step(dense_rows(x), dense_rows(gate),
-                                              state, out, act)
-        return y, out
     y, new = gated_scan_torch(x[:, None], gate[:, None], state, act=act)
     return y[:, 0], state.copy_(new) if inplace else new
 

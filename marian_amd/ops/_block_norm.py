@@ -1,6 +1,6 @@
-"""The join of two transformer blocks (norm, gate, residual, next norm):
-argument checks, the autograd wrapper of the HIP kernels and the plain
-composite used off the GPU.
+"""The join of two transformer blocks (norm, gate, residual, next norm) off
+the GPU: argument checks and the plain composite. On the GPU the extension
+checks the same and runs the kernels.
 
 ref: models/transformer.h preProcess/postProcess ('n', 'a') and the highway
 functor (out = sigmoid(t) in1 + (1 - sigmoid(t)) in2).
@@ -8,19 +8,15 @@ functor (out = sigmoid(t) in1 + (1 - sigmoid(t)) in2).
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
-
-from . import hip_ext
 
 MAX_WIDTH = 16384
-_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16, torch.float64)
 
 
 def check_join(x, res, gate, gate_kind, params, norm):
     """params: {name: tensor or None} of the four norm parameters."""
-    ok = _DTYPES if x.is_cuda else _DTYPES + (torch.float64,)
-    if x.dim() < 1 or x.dtype not in ok:
-        raise ValueError(f"block_norm: x must be [..., D] of {ok}, got "
+    if x.dim() < 1 or x.dtype not in _DTYPES:
+        raise ValueError(f"block_norm: x must be [..., D] of {_DTYPES}, got "
                          f"{x.dtype} {tuple(x.shape)}")
     D = x.shape[-1]
     if not 0 < D <= MAX_WIDTH:
@@ -84,32 +80,3 @@ def block_norm_torch(x, res, gate=None, gate_kind="scale", res_scale=1.0,
     h = None if pre_scale is None else normed(s, pre_scale, pre_bias).to(
         x.dtype)
     return s.to(x.dtype), h
-
-
-class BlockNormFn(torch.autograd.Function):
-    """x and res as [R, D]; returns (s, h) with h empty without pre_scale."""
-
-    @staticmethod
-    def forward(ctx, x, res, gate, post_scale, post_bias, pre_scale, pre_bias,
-                highway, alpha, rms, eps):
-        want = any(ctx.needs_input_grad)
-        s, h, stat = hip_ext(required=True).block_norm_fwd(
-            x, res, gate, highway, alpha, post_scale, post_bias, pre_scale,
-            pre_bias, rms, eps, want)
-        if want:
-            ctx.save_for_backward(x, res, gate, post_scale, post_bias,
-                                  pre_scale, pre_bias, stat)
-            ctx.conf = (highway, alpha, rms, eps)
-            ctx.set_materialize_grads(False)
-        return s, h
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, ds, dh):
-        x, res, gate, w1, b1, w2, b2, stat = ctx.saved_tensors
-        highway, alpha, rms, eps = ctx.conf
-        want = list(ctx.needs_input_grad[:7])
-        outs = hip_ext(required=True).block_norm_bwd(
-            x, res, gate, highway, alpha, w1, b1, w2, b2, rms, eps, stat, ds,
-            dh, want)
-        return tuple(o if w else None for o, w in zip(outs, want)) + (None,) * 4

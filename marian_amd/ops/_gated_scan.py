@@ -1,16 +1,13 @@
-"""Gated linear recurrence (SSRU): argument checks, the autograd wrapper of
-the HIP kernels and the plain composite used off the GPU.
+"""Gated linear recurrence (SSRU) off the GPU: argument checks and the plain
+composite. On the GPU the extension checks the same and runs the kernels.
 
 ref: src/rnn/cells.h SSRU (f = sigmoid(Wf x + bf), highway(cell, W x, f)).
 """
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from . import hip_ext
-
-_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16, torch.float64)
 _ACTS = ("none", "relu")
 
 
@@ -26,8 +23,7 @@ def check_scan(what, x, gate, state, lens, act, dims):
         raise ValueError(f"{what}: x and gate must share dtype and device")
     if x.shape[-1] == 0:
         raise ValueError(f"{what}: the width must be positive")
-    ok = _DTYPES if x.is_cuda else _DTYPES + (torch.float64,)
-    if x.dtype not in ok:
+    if x.dtype not in _DTYPES:
         raise ValueError(f"{what}: unsupported dtype {x.dtype}")
     if act not in _ACTS:
         raise ValueError(f"{what}: act must be one of {_ACTS}, got {act!r}")
@@ -42,16 +38,6 @@ def check_scan(what, x, gate, state, lens, act, dims):
             or lens.device != x.device):
         raise ValueError(f"{what}: lens must be int32 {(x.shape[0],)} on x's "
                          "device")
-
-
-def dense_rows(t):
-    """t, or a copy of it if its last dimension is not dense or its rows lie
-    further apart than the kernels' offsets reach."""
-    if t.stride(-1) != 1 and t.shape[-1] != 1:
-        return t.contiguous()
-    if t.dim() == 3 and t.shape[1] > 1 and t.stride(1) >= 1 << 26:
-        return t.contiguous()
-    return t
 
 
 def gated_scan_torch(x, gate, state=None, lens=None, reverse=False,
@@ -73,62 +59,3 @@ def gated_scan_torch(x, gate, state=None, lens=None, reverse=False,
         c, ys[t] = new, out
     y = torch.stack(ys, dim=1) if T else om * xa
     return y.to(x.dtype), c
-
-
-class GatedScanFn(torch.autograd.Function):
-    """x and gate as two tensors."""
-
-    @staticmethod
-    def forward(ctx, x, gate, state, lens, reverse, act):
-        return _forward(ctx, x, gate, (x, gate), state, lens, reverse, act)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dlast):
-        x, gate = ctx.saved_tensors[:2]
-        dx = torch.empty_like(x, memory_format=torch.contiguous_format)
-        dg = torch.empty_like(gate, memory_format=torch.contiguous_format)
-        ds = _backward(ctx, x, gate, dy, dlast, dx, dg, 2)
-        return dx, dg, ds, None, None, None
-
-
-class GatedScanXGFn(torch.autograd.Function):
-    """x and gate as the halves of one fused projection: one buffer in, one
-    gradient buffer out."""
-
-    @staticmethod
-    def forward(ctx, xg, state, lens, reverse, act):
-        d = xg.shape[-1] // 2
-        return _forward(ctx, xg[..., :d], xg[..., d:], (xg,), state, lens,
-                        reverse, act)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dlast):
-        xg = ctx.saved_tensors[0]
-        d = xg.shape[-1] // 2
-        dxg = torch.empty_like(xg, memory_format=torch.contiguous_format)
-        ds = _backward(ctx, xg[..., :d], xg[..., d:], dy, dlast,
-                       dxg[..., :d], dxg[..., d:], 1)
-        return dxg, ds, None, None, None
-
-
-def _forward(ctx, x, gate, saved, state, lens, reverse, act):
-    want = any(ctx.needs_input_grad)
-    y, last, bnd = hip_ext(required=True).gated_scan_fwd(
-        x, gate, state, lens, reverse, act, want)
-    if want:
-        ctx.save_for_backward(*saved, state, lens, bnd)
-        ctx.reverse, ctx.act = reverse, act
-        ctx.want_dstate = state is not None and state.requires_grad
-        ctx.set_materialize_grads(False)
-    return y, last
-
-
-def _backward(ctx, x, gate, dy, dlast, dx, dg, n):
-    state, lens, bnd = ctx.saved_tensors[n:]
-    ds = hip_ext(required=True).gated_scan_bwd(
-        x, gate, state, lens, bnd, dy,
-        None if dlast is None else dlast.contiguous(), ctx.reverse, ctx.act,
-        dx, dg, ctx.want_dstate)
-    return ds if ctx.want_dstate else None

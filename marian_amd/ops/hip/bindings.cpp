@@ -56,37 +56,22 @@ std::vector<torch::Tensor> attention_bwd(torch::Tensor q, torch::Tensor k,
                                          c10::optional<torch::Tensor> kv_lens,
                                          bool causal, double scale);
 
-std::vector<torch::Tensor> gated_scan_fwd(torch::Tensor x, torch::Tensor gate,
-                                          c10::optional<torch::Tensor> state,
-                                          c10::optional<torch::Tensor> lens,
-                                          bool reverse, std::string act,
-                                          bool want_bnd);
-torch::Tensor gated_scan_bwd(torch::Tensor x, torch::Tensor gate,
-                             c10::optional<torch::Tensor> state,
-                             c10::optional<torch::Tensor> lens,
-                             torch::Tensor bnd,
-                             c10::optional<torch::Tensor> dy,
-                             c10::optional<torch::Tensor> dlast, bool reverse,
-                             std::string act, torch::Tensor dx,
-                             torch::Tensor dgate, bool want_dstate);
-torch::Tensor gated_step(torch::Tensor x, torch::Tensor gate,
-                         torch::Tensor state, torch::Tensor state_out,
-                         std::string act);
-std::vector<torch::Tensor> block_norm_fwd(
+std::tuple<torch::Tensor, torch::Tensor> gated_scan(
+    torch::Tensor x, torch::Tensor gate, c10::optional<torch::Tensor> state,
+    c10::optional<torch::Tensor> lens, bool reverse, std::string act);
+std::tuple<torch::Tensor, torch::Tensor> gated_scan_xg(
+    torch::Tensor xg, c10::optional<torch::Tensor> state,
+    c10::optional<torch::Tensor> lens, bool reverse, std::string act);
+std::tuple<torch::Tensor, torch::Tensor> gated_step(
+    torch::Tensor x, torch::Tensor gate, c10::optional<torch::Tensor> state,
+    std::string act, bool inplace);
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> block_norm(
     torch::Tensor x, torch::Tensor res, c10::optional<torch::Tensor> gate,
-    bool highway, double alpha, c10::optional<torch::Tensor> post_scale,
+    std::string gate_kind, double alpha,
+    c10::optional<torch::Tensor> post_scale,
     c10::optional<torch::Tensor> post_bias,
     c10::optional<torch::Tensor> pre_scale,
-    c10::optional<torch::Tensor> pre_bias, bool rms, double eps,
-    bool want_stat);
-std::vector<torch::Tensor> block_norm_bwd(
-    torch::Tensor x, torch::Tensor res, c10::optional<torch::Tensor> gate,
-    bool highway, double alpha, c10::optional<torch::Tensor> post_scale,
-    c10::optional<torch::Tensor> post_bias,
-    c10::optional<torch::Tensor> pre_scale,
-    c10::optional<torch::Tensor> pre_bias, bool rms, double eps,
-    torch::Tensor stat, c10::optional<torch::Tensor> dsum,
-    c10::optional<torch::Tensor> dh, std::vector<bool> want);
+    c10::optional<torch::Tensor> pre_bias, std::string norm, double eps);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layernorm_fwd", &layernorm_fwd, "LayerNorm forward (gfx950)");
@@ -130,13 +115,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sumsq_finite", &sumsq_finite, "fused grad sumsq + nonfinite count");
   m.def("beam_topk", &beam_topk,
         "fused beam-search top-k (path-score add + UNK suppression)");
-  m.def("gated_scan_fwd", &gated_scan_fwd,
-        "gated linear recurrence over sequences");
-  m.def("gated_scan_bwd", &gated_scan_bwd,
-        "its gradient, written into given strided views");
+  m.def("gated_scan", &gated_scan,
+        "gated linear recurrence over sequences (autograd)");
+  m.def("gated_scan_xg", &gated_scan_xg,
+        "gated linear recurrence on a fused projection (autograd)");
   m.def("gated_step", &gated_step,
         "gated linear recurrence, one token per row");
-  m.def("block_norm_fwd", &block_norm_fwd,
-        "fused norm, gate, residual and next norm of a block");
-  m.def("block_norm_bwd", &block_norm_bwd, "its gradient");
+  m.def("block_norm", &block_norm,
+        "fused norm, gate, residual and next norm of a block (autograd)");
 }

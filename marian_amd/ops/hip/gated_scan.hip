@@ -625,12 +625,6 @@ __global__ __launch_bounds__(256) void step_kernel(
   }
 }
 
-int act_code(const std::string& act) {
-  TORCH_CHECK(act == "none" || act == "relu",
-              "gated_scan: act must be none or relu, got ", act);
-  return act == "relu";
-}
-
 void check_rows(const torch::Tensor& x, const torch::Tensor& g,
                 const char* what) {
   TORCH_CHECK(x.is_cuda() && g.device() == x.device(), what,
@@ -679,7 +673,7 @@ long time_stride(const torch::Tensor& t) {
 ScanArgs base_args(const torch::Tensor& x, const torch::Tensor& g,
                    const c10::optional<torch::Tensor>& state,
                    const c10::optional<torch::Tensor>& lens, bool reverse,
-                   const std::string& act) {
+                   bool relu) {
   check_rows(x, g, "gated_scan");
   TORCH_CHECK(x.dim() == 3, "gated_scan: x must be [B, T, D]");
   TORCH_CHECK(x.size(0) < (1 << 30) && x.size(1) < (1 << 30) &&
@@ -708,7 +702,7 @@ ScanArgs base_args(const torch::Tensor& x, const torch::Tensor& g,
   a.nc = std::max((a.nt + a.tpc - 1) / a.tpc, 1);
   TORCH_CHECK(pairs < (1L << 31), "gated_scan: too many rows");
   a.reverse = reverse;
-  a.relu = act_code(act);
+  a.relu = relu;
   return a;
 }
 
@@ -763,9 +757,9 @@ void run(bool bwd, const torch::Tensor& x, ScanArgs& a) {
 std::vector<torch::Tensor> gated_scan_fwd(torch::Tensor x, torch::Tensor gate,
                                           c10::optional<torch::Tensor> state,
                                           c10::optional<torch::Tensor> lens,
-                                          bool reverse, std::string act,
+                                          bool reverse, bool relu,
                                           bool want_bnd) {
-  ScanArgs a = base_args(x, gate, state, lens, reverse, act);
+  ScanArgs a = base_args(x, gate, state, lens, reverse, relu);
   const c10::DeviceGuard guard(x.device());
   auto f32 = x.options().dtype(torch::kFloat32);
   auto y = torch::empty({a.B, a.T, a.D}, x.options());
@@ -790,9 +784,9 @@ torch::Tensor gated_scan_bwd(torch::Tensor x, torch::Tensor gate,
                              torch::Tensor bnd,
                              c10::optional<torch::Tensor> dy,
                              c10::optional<torch::Tensor> dlast, bool reverse,
-                             std::string act, torch::Tensor dx,
+                             bool relu, torch::Tensor dx,
                              torch::Tensor dgate, bool want_dstate) {
-  ScanArgs a = base_args(x, gate, state, lens, reverse, act);
+  ScanArgs a = base_args(x, gate, state, lens, reverse, relu);
   const c10::DeviceGuard guard(x.device());
   check_rows(dx, dgate, "gated_scan_bwd");
   TORCH_CHECK(dx.sizes() == x.sizes() && dx.device() == x.device() &&
@@ -830,12 +824,11 @@ torch::Tensor gated_scan_bwd(torch::Tensor x, torch::Tensor gate,
 }
 
 // one step for N rows; state_out may be state itself
-torch::Tensor gated_step(torch::Tensor x, torch::Tensor gate,
-                         torch::Tensor state, torch::Tensor state_out,
-                         std::string act) {
+torch::Tensor gated_step_fwd(torch::Tensor x, torch::Tensor gate,
+                             torch::Tensor state, torch::Tensor state_out,
+                             bool relu) {
   check_rows(x, gate, "gated_step");
   TORCH_CHECK(x.dim() == 2, "gated_step: x must be [N, D]");
-  const int relu = act_code(act);
   const float* sp = state_ptr(state, x, "state");
   state_ptr(state_out, x, "state_out");
   const c10::DeviceGuard guard(x.device());

@@ -36,7 +36,7 @@ fp8q = os.path.join(HIP_DIR, "fp8q.hip")
 if os.path.exists(fp8q):
     sources.append(fp8q)
 for name in ("gated_scan.hip", "block_norm.hip", "block_norm_bf16.hip",
-             "block_norm_f16.hip", "block_norm_f32.hip"):
+             "block_norm_f16.hip", "block_norm_f32.hip", "block_ops.cpp"):
     if os.path.exists(os.path.join(HIP_DIR, name)):
         sources.append(os.path.join(HIP_DIR, name))
 ltgemm = os.path.join(HIP_DIR, "ltgemm.cpp")

@@ -198,8 +198,11 @@ def test_plain_gradients_by_differences(norm, gate):
         fn, [t[k].clone().requires_grad_() for k in keys])
 
 
-def test_refusals():
-    x, w = torch.zeros(2, 3, 4), torch.ones(4)
+@pytest.mark.parametrize("dev", ["cpu", pytest.param(
+    "cuda", marks=pytest.mark.gpu)])
+def test_refusals(dev):
+    x, w = torch.zeros(2, 3, 4, device=dev), torch.ones(4, device=dev)
+    zeros = lambda *s: torch.zeros(*s, device=dev)
 
     def refused(*a, **k):
         with pytest.raises(ValueError):
@@ -208,19 +211,23 @@ def test_refusals():
     refused(x, x.bfloat16())
     refused(x.long(), x.long())
     refused(x[..., :0], x[..., :0])
-    refused(torch.zeros(()), torch.zeros(()))
-    refused(torch.zeros(1, 16385), torch.zeros(1, 16385))
+    refused(zeros(()), zeros(()))
+    refused(zeros(1, 16385), zeros(1, 16385))
     refused(x, x, norm="batch")
     refused(x, x, gate_kind="tanh")
     refused(x, x, gate=w[:3])
-    refused(x, x, gate=torch.zeros(3, 4))
-    refused(x, x, gate=torch.zeros(2, 1, 4))
-    refused(x, x, gate=torch.zeros(2, 3, 4).bfloat16())
+    refused(x, x, gate=zeros(3, 4))
+    refused(x, x, gate=zeros(2, 1, 4))
+    refused(x, x, gate=zeros(2, 3, 4).bfloat16())
     refused(x, x, post_bias=w)
     refused(x, x, pre_scale=w[:3])
     refused(x, x, pre_scale=w.double())
     refused(x, x, pre_scale=w, pre_bias=w.bfloat16())
     refused(x, x, pre_scale=w[None])
+    if dev == "cuda":
+        refused(x, x.cpu())
+        refused(x, x, pre_scale=w.cpu())
+        refused(x.double(), x.double())
 
 
 # ------------------------------------------------------------------ on the GPU
@@ -316,6 +323,16 @@ def test_gpu_partial_gradients():
         g, = torch.autograd.grad(call(r, "layer", "highway", 1.0), r[k],
                                  (t["dsum"], t["dh"]))
         assert torch.equal(g, full[k]), k
+
+
+@pytest.mark.gpu
+def test_gpu_is_differentiable_once():
+    t = make(4, 32, torch.float32, "cuda", gate="scale")
+    t["x"].requires_grad_()
+    g, = torch.autograd.grad(call(t, "layer", "scale", 1.0)[1], t["x"],
+                             t["dh"], create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        g.sum().backward()
 
 
 @pytest.mark.gpu

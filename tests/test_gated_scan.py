@@ -190,9 +190,15 @@ def _refused(fn, *a, **k):
         fn(*a, **k)
 
 
-def test_scan_refusals():
-    x = torch.zeros(2, 3, 4)
-    s = torch.zeros(2, 4)
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_scan_refusals(dev):
+    x = torch.zeros(2, 3, 4, device=dev)
+    s = torch.zeros(2, 4, device=dev)
+    zeros = lambda n, dtype=torch.float32: torch.zeros(n, dtype=dtype,
+                                                       device=dev)
     _refused(ops.gated_scan, x[0], x[0])
     _refused(ops.gated_scan, x, x[:, :2])
     _refused(ops.gated_scan, x, x.bfloat16())
@@ -201,20 +207,27 @@ def test_scan_refusals():
     _refused(ops.gated_scan, x, x, act="tanh")
     _refused(ops.gated_scan, x, x, state=s.bfloat16())
     _refused(ops.gated_scan, x, x, state=s[:1])
-    _refused(ops.gated_scan, x, x, lens=torch.zeros(2))
-    _refused(ops.gated_scan, x, x, lens=torch.zeros(3, dtype=torch.int32))
-    _refused(ops.gated_scan, x, x, lens=torch.zeros(2, dtype=torch.int64))
+    _refused(ops.gated_scan, x, x, lens=zeros(2))
+    _refused(ops.gated_scan, x, x, lens=zeros(3, torch.int32))
+    _refused(ops.gated_scan, x, x, lens=zeros(2, torch.int64))
+    if dev == "cuda":
+        _refused(ops.gated_scan, x, x.cpu())
+        _refused(ops.gated_scan, x, x, state=s.cpu())
+        _refused(ops.gated_scan, x, x, lens=zeros(2, torch.int32).cpu())
+        _refused(ops.gated_scan, x.double(), x.double())
     _refused(ops.gated_scan_xg, x[..., :3])
     _refused(ops.gated_scan_xg, x[0])
 
 
-def test_step_refusals():
-    x, s = torch.zeros(2, 4), torch.zeros(2, 4)
+@pytest.mark.parametrize("dev", DEVICES)
+def test_step_refusals(dev):
+    x, s = torch.zeros(2, 4, device=dev), torch.zeros(2, 4, device=dev)
     _refused(ops.gated_step, x, x, None)
     _refused(ops.gated_step, x[:, None], x[:, None], s)
     _refused(ops.gated_step, x, x, s[:1])
     _refused(ops.gated_step, x, x, s.half())
-    _refused(ops.gated_step, x, x, torch.zeros(4, 2).t(), inplace=True)
+    _refused(ops.gated_step, x, x, torch.zeros(4, 2, device=dev).t(),
+             inplace=True)
     _refused(ops.gated_step, x.requires_grad_(), x, s, inplace=True)
 
 
@@ -314,6 +327,16 @@ def test_scan_gpu_partial_gradients():
     a = torch.autograd.grad(ops.gated_scan(x, g)[0].sum(), x)
     b = torch.autograd.grad(ops.gated_scan(x, g)[0], x, torch.ones_like(dy))
     assert torch.equal(a[0], b[0])
+
+
+@pytest.mark.gpu
+def test_scan_gpu_is_differentiable_once():
+    xg, st, _, dy, _ = make(2, 5, 6, torch.float32, "cuda", 3)
+    xg.requires_grad_()
+    g, = torch.autograd.grad(ops.gated_scan_xg(xg, st)[0], xg, dy,
+                             create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        g.sum().backward()
 
 
 @pytest.mark.gpu
