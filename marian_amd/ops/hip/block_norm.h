@@ -29,14 +29,27 @@
 // The kernels are instantiated per element type, a source file each.
 #pragma once
 
+#include <atomic>
+
 #include "common.h"
 #include "vec.h"
 
 namespace mamd {
 
-enum { kGateNone = 0, kGateChannel = 1, kGateToken = 2 };
-// the parameter gradients' rows in a block's partial sums
-enum { kPostScale = 0, kPostBias, kPreScale, kPreBias, kGate, kNumParams };
+// gates: per channel or per token, a factor or a highway's logit
+enum { kNone = 0, kScaleCh, kScaleTok, kHighCh, kHighTok };
+constexpr bool is_highway(int g) { return g == kHighCh || g == kHighTok; }
+constexpr bool is_channel(int g) { return g == kScaleCh || g == kHighCh; }
+constexpr bool is_token(int g) { return g == kScaleTok || g == kHighTok; }
+
+// Sums over rows that the parameter gradients are made of, xh and sh the
+// normalised rows (xh = x without a post norm):
+//   dpre_scale = P1, dpre_bias = P0, dpost_scale = b S1, dpost_bias = b S0,
+//   dgate = w1 S1 + b1 S0                       (scale, per channel)
+//           k (1-k) (w1 S1 + b1 S0 - alpha S2)  (highway, per channel)
+// since b, w1 and b1 do not change along the rows; so a channel gate costs no
+// accumulators of its own. With a gate per token S1 and S0 take b inside.
+enum { kS1 = 0, kS0, kS2, kP1, kP0, kNumSums };
 
 struct NormArgs {
   const void* x;
@@ -47,7 +60,7 @@ struct NormArgs {
   const void* pre_scale;
   const void* pre_bias;
   int param32;               // parameters are float32 rather than x's type
-  int rms, highway;
+  int rms;
   float alpha, eps;
   long rows;
   int D;
@@ -61,25 +74,50 @@ struct NormArgs {
   const void* dh;
   void* dx;                  // any of these may be null
   void* dres;
-  void* dgate;               // kGateToken only
+  void* dgate;               // per token
   float* part;               // [blocks][n_part][D] or null
   int n_part;
-  int slot[kNumParams];      // a parameter's row in part, or -1
+  int slot[kNumSums];        // a sum's row in part, or -1
 };
 
-// sums of two values over the lanes of a row, given to all of them. Rows of
-// more than a wave meet in LDS; alternating between two buffers makes one
-// barrier enough.
+// How a row's lanes are placed: some lanes of a wave, one wave, or a block.
+enum { kPartWave = 0, kWave = 1, kBlock = 2 };
+
+// sum over a wave in a fixed order, in all lanes: 4 steps inside rows of 16
+// lanes and 2 between them, all of them modifiers of an add
+__device__ __forceinline__ float dpp_sum(float v) {
+#define STEP(CTRL, ROWS)                                                  \
+  v += __int_as_float(__builtin_amdgcn_update_dpp(                        \
+      0, __float_as_int(v), CTRL, ROWS, 0xf, true))
+  STEP(0x111, 0xf);  // row_shr:1
+  STEP(0x112, 0xf);
+  STEP(0x114, 0xf);
+  STEP(0x118, 0xf);
+  STEP(0x142, 0xa);  // row_bcast:15 into rows 1 and 3
+  STEP(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
+#undef STEP
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+// sums of two values over the lanes of a row, given to all of them. The waves
+// of a block meet in LDS; alternating between two buffers makes one barrier
+// enough.
+template <int PLACE>
 struct RowSum {
   float (*buf)[32];
   int tpr, flip;
   __device__ RowSum(float (*b)[32], int t) : buf(b), tpr(t), flip(0) {}
   __device__ __forceinline__ void operator()(float& p, float& q) {
-    for (int off = min(tpr, WAVE) >> 1; off > 0; off >>= 1) {
-      p += __shfl_xor(p, off, WAVE);
-      q += __shfl_xor(q, off, WAVE);
+    if constexpr (PLACE == kPartWave) {
+      for (int off = tpr >> 1; off > 0; off >>= 1) {
+        p += __shfl_xor(p, off, WAVE);
+        q += __shfl_xor(q, off, WAVE);
+      }
+    } else {
+      p = dpp_sum(p);
+      q = dpp_sum(q);
     }
-    if (tpr > WAVE) {  // one row per block
+    if constexpr (PLACE == kBlock) {
       const int nw = tpr / WAVE, wid = threadIdx.x / WAVE;
       if (threadIdx.x % WAVE == 0)
         buf[flip][wid] = p, buf[flip][16 + wid] = q;
@@ -89,167 +127,263 @@ struct RowSum {
       flip ^= 1;
     }
   }
+  __device__ __forceinline__ void operator()(float& p) {
+    if constexpr (PLACE == kWave) {
+      p = dpp_sum(p);
+    } else {
+      float q = 0.f;
+      (*this)(p, q);
+    }
+  }
 };
 
-template <typename T, int VEC>
-__device__ __forceinline__ void load_f32(const T* p, int n, float* o) {
-  if (n >= VEC) {
-    const vec_t<T, VEC> r = load_vec<T, VEC>(p);
+// A lane's columns: NC vectors of VEC, `step` apart. A vector that would pass
+// the row's end moves back to the row's last VEC columns: it computes what its
+// neighbour computes and writes the same values there, but the columns that it
+// has twice (those before `first`) stay out of every sum.
+template <int VEC, int NC>
+struct Columns {
+  int at[NC], first[NC];
+  __device__ __forceinline__ Columns(int lane, int tpr, int D) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) o[i] = (float)r[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) o[i] = i < n ? (float)p[i] : 0.f;
+    for (int i = 0; i < NC; ++i) {
+      first[i] = (lane + i * tpr) * VEC;
+      at[i] = min(first[i], D - VEC);
+    }
   }
+  __device__ __forceinline__ bool own(int e) const {
+    return at[e / VEC] + e % VEC >= first[e / VEC];
+  }
+  __device__ __forceinline__ bool any(int i, int D) const {
+    return first[i] < D;
+  }
+};
+
+template <typename T, int VEC, int NC>
+struct RawRow {
+  vec_t<T, VEC> r[NC];
+  __device__ __forceinline__ void load(const T* p,
+                                       const Columns<VEC, NC>& c) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) r[i] = load_vec<T, VEC>(p + c.at[i]);
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) r[i] = {};
+  }
+  __device__ __forceinline__ float operator[](int e) const {
+    return (float)r[e / VEC][e % VEC];
+  }
+};
+
+template <typename V>
+__device__ __forceinline__ V opaque(V v) {
+  if constexpr (sizeof(V) % 4 == 0) {
+    unsigned w[sizeof(V) / 4];
+    __builtin_memcpy(w, &v, sizeof(V));
+#pragma unroll
+    for (unsigned& x : w) asm("" : "+v"(x));
+    __builtin_memcpy(&v, w, sizeof(V));
+  }
+  return v;
 }
 
-template <typename T, int VEC>
-__device__ __forceinline__ void store_f32(T* p, int n, const float* o) {
-  if (n >= VEC) {
-    store_vec<T, VEC>(p, o);
-  } else {
+// A parameter vector's columns. KEEP: those of x's type stay in registers, in
+// that type, over the rows of a block (the empty asm keeps the compiler from
+// holding their 32-bit values instead, twice the registers). Others - float32
+// ones beside 16-bit rows - are read again for each row, from L1 or L2.
+template <typename T, int VEC, int NC, bool KEEP>
+struct Param {
+  const void* p;
+  int wide;
+  float dflt;
+  RawRow<T, VEC, KEEP ? NC : 1> raw;
+  __device__ __forceinline__ Param(const void* p_, int param32, float d,
+                                   const Columns<VEC, NC>& c)
+      : p(p_), wide(param32 && sizeof(T) != 4), dflt(d) {
+    if constexpr (KEEP) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i)
-      if (i < n) p[i] = (T)o[i];
-  }
-}
-
-// a parameter vector, whose type may be x's or float32; null: the default
-template <typename T, int VEC>
-__device__ __forceinline__ void load_param(const void* p, int param32, int c,
-                                           int n, float dflt, float* o) {
-  if (!p) {
+      for (int i = 0; i < NC; ++i)
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) o[i] = dflt;
-  } else if (param32) {
-    load_f32<float, VEC>((const float*)p + c, n, o);
-  } else {
-    load_f32<T, VEC>((const T*)p + c, n, o);
+        for (int v = 0; v < VEC; ++v) raw.r[i][v] = (T)d;
+      if (p && !wide) raw.load((const T*)p, c);
+    }
   }
-}
-
-// EPT elements per lane in chunks of 16 bytes
-template <typename T>
-constexpr int vec_of() { return 16 / (int)sizeof(T); }
-
-template <typename T, int EPT, int GATE>
-__device__ __forceinline__ void load_gate(const NormArgs& a, long row, int c0,
-                                          int step, float* gt) {
-  constexpr int VEC = vec_of<T>(), NC = EPT / VEC;
+  __device__ __forceinline__ void get(const Columns<VEC, NC>& c,
+                                      float o[VEC * NC]) const {
+    if (KEEP && !(sizeof(T) != 4 && wide)) {
 #pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const int c = c0 + i * step, n = a.D - c;
-    if constexpr (GATE == kGateToken)
-      load_f32<T, VEC>((const T*)a.gate + row * a.D + c, n, gt + i * VEC);
-    else
-      load_param<T, VEC>(a.gate, a.param32, c, n, 0.f, gt + i * VEC);
+      for (int i = 0; i < NC; ++i) {
+        const vec_t<T, VEC> r = opaque(raw.r[KEEP ? i : 0]);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) o[i * VEC + v] = (float)r[v];
+      }
+    } else if (!p) {
+#pragma unroll
+      for (int e = 0; e < VEC * NC; ++e) o[e] = dflt;
+    } else if (sizeof(T) != 4 && wide) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const vec_t<float, VEC> w =
+            load_vec<float, VEC>((const float*)p + c.at[i]);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) o[i * VEC + v] = w[v];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const vec_t<T, VEC> w = load_vec<T, VEC>((const T*)p + c.at[i]);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) o[i * VEC + v] = (float)w[v];
+      }
+    }
   }
-}
+};
 
 // coefficients of res and u; k is the highway gate's sigmoid
 template <typename T, int GATE>
-__device__ __forceinline__ void coefs(const NormArgs& a, float gt, float& ca,
-                                      float& cb, float& k, float& k1) {
-  ca = a.alpha, cb = 1.f, k = 0.f, k1 = 1.f;
-  if constexpr (GATE != kGateNone) {
-    if (a.highway) {
-      sigmoid2<T>(gt, k, k1);
-      ca = a.alpha * k1, cb = k;
-    } else {
-      cb = gt;
-    }
+__device__ __forceinline__ void coefs(float alpha, float gt, float& ca,
+                                      float& cb, float& k1) {
+  ca = alpha, cb = 1.f, k1 = 1.f;
+  if constexpr (is_highway(GATE)) {
+    sigmoid2<T>(gt, cb, k1);
+    ca = alpha * k1;
+  } else if constexpr (GATE != kNone) {
+    cb = gt;
   }
 }
 
-// mean and 1/deviation of the elements that exist
-template <int EPT, int VEC>
-__device__ __forceinline__ void stats(const float* v, int c0, int step, int D,
-                                      int rms, float eps, RowSum& sum,
+// mean and 1/deviation of a row
+template <int VEC, int NC, int PLACE>
+__device__ __forceinline__ void stats(const float* v,
+                                      const Columns<VEC, NC>& c, int D,
+                                      int rms, float eps, RowSum<PLACE>& sum,
                                       float& mean, float& rstd) {
-  float p = 0.f, q = 0.f;
   mean = 0.f;
   if (!rms) {
+    float p = 0.f;
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) p += v[i];  // absent elements are 0
-    sum(p, q);
+    for (int e = 0; e < VEC * NC; ++e) p += c.own(e) ? v[e] : 0.f;
+    sum(p);
     mean = p / D;
   }
-  q = p = 0.f;
+  float q = 0.f;
 #pragma unroll
-  for (int i = 0; i < EPT; ++i) {
-    const float e = v[i] - mean;
-    q += c0 + (i / VEC) * step + i % VEC < D ? e * e : 0.f;
+  for (int e = 0; e < VEC * NC; ++e) {
+    const float d = c.own(e) ? v[e] - mean : 0.f;
+    q += d * d;
   }
-  sum(q, p);
+  sum(q);
   rstd = 1.f / sqrtf(q / D + eps);
 }
 
-template <typename T, int EPT, bool POST, bool PRE, int GATE, int MAXT>
-__global__ __launch_bounds__(MAXT) void join_fwd_kernel(NormArgs a) {
-  constexpr int VEC = vec_of<T>(), NC = EPT / VEC;
-  __shared__ float buf[2][32];
-  RowSum sum(buf, a.tpr);
-  const int lane = threadIdx.x & (a.tpr - 1);
-  const int rpb = max((int)blockDim.x / a.tpr, 1);
-  const int c0 = lane * VEC, step = a.tpr * VEC;
-  for (long r0 = (long)blockIdx.x * rpb; r0 < a.rows;
-       r0 += (long)gridDim.x * rpb) {
-    long row = r0 + threadIdx.x / a.tpr;
-    const bool on = row < a.rows;
-    if (!on) row = a.rows - 1;  // its lanes work along and store nothing
-    const long base = row * a.D;
-    float x[EPT], s[EPT], gt[EPT];
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int c = c0 + i * step;
-      load_f32<T, VEC>((const T*)a.x + base + c, a.D - c, x + i * VEC);
-      load_f32<T, VEC>((const T*)a.res + base + c, a.D - c, s + i * VEC);
+// the rows of a lane group, and the next of them
+template <int PLACE>
+struct Rows {
+  long row, stride;
+  int lane;
+  __device__ __forceinline__ Rows(const NormArgs& a) {
+    if constexpr (PLACE == kPartWave) {
+      const int rpb = blockDim.x / a.tpr;
+      lane = threadIdx.x & (a.tpr - 1);
+      row = (long)blockIdx.x * rpb + threadIdx.x / a.tpr;
+      stride = (long)gridDim.x * rpb;
+    } else if constexpr (PLACE == kWave) {
+      const int rpb = blockDim.x / WAVE;
+      lane = threadIdx.x & (WAVE - 1);
+      row = (long)blockIdx.x * rpb +
+            __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+      stride = (long)gridDim.x * rpb;
+    } else {
+      lane = threadIdx.x;
+      row = blockIdx.x;
+      stride = gridDim.x;
     }
-    if constexpr (GATE != kGateNone)
-      load_gate<T, EPT, GATE>(a, row, c0, step, gt);
+  }
+};
+
+// Lanes without a row (the end of the last block, part-wave placement only
+// mixes them with others) work on the last row and store nothing; sums never
+// leave a lane group, so they cost the others nothing but time.
+template <typename T, int VEC, int EPT, int PLACE, bool POST, bool PRE,
+          int GATE, int MAXT>
+__global__ __launch_bounds__(MAXT) void join_fwd_kernel(NormArgs a) {
+  constexpr int NC = EPT / VEC;
+  // blocks of 1024 have 128 registers a lane: parameters are read again for
+  // each row and nothing is fetched ahead
+  constexpr bool KEEP = MAXT <= 512;
+  using Raw = RawRow<T, VEC, NC>;
+  __shared__ float buf[2][32];
+  RowSum<PLACE> sum(buf, a.tpr);
+  const Rows<PLACE> it(a);
+  const Columns<VEC, NC> col(it.lane, a.tpr, a.D);
+  const Param<T, VEC, NC, KEEP> w1(POST ? a.post_scale : nullptr, a.param32, 1.f,
+                             col);
+  const Param<T, VEC, NC, KEEP> b1(POST ? a.post_bias : nullptr, a.param32, 0.f,
+                             col);
+  const Param<T, VEC, NC, KEEP> w2(PRE ? a.pre_scale : nullptr, a.param32, 1.f, col);
+  const Param<T, VEC, NC, KEEP> b2(PRE ? a.pre_bias : nullptr, a.param32, 0.f, col);
+  const Param<T, VEC, NC, KEEP> gp(is_channel(GATE) ? a.gate : nullptr,
+                             a.param32, 0.f, col);
+
+  Raw xr, rr, gr;
+  auto fetch = [&](long row) __attribute__((always_inline)) {
+    const long base = min(row, a.rows - 1) * a.D;
+    xr.load((const T*)a.x + base, col);
+    rr.load((const T*)a.res + base, col);
+    if constexpr (is_token(GATE)) gr.load((const T*)a.gate + base, col);
+  };
+  if (KEEP) fetch(it.row);
+  // the same number of turns for all lanes of a wave
+  for (long r0 = 0, n = (a.rows + it.stride - 1) / it.stride; r0 < n; ++r0) {
+    const long row = it.row + r0 * it.stride;
+    if (PLACE != kPartWave && row >= a.rows) break;
+    if (!KEEP) fetch(row);
+    const bool on = row < a.rows;
+    const long base = row * a.D;
+    float x[EPT], s[EPT], gt[EPT], w[EPT], bb[EPT];
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) {
+      x[e] = xr[e];
+      s[e] = rr[e];
+      gt[e] = is_token(GATE) ? gr[e] : 0.f;
+    }
+    if (KEEP && r0 + 1 < n) fetch(row + it.stride);
+    if constexpr (is_channel(GATE)) gp.get(col, gt);
     float m1 = 0.f, r1 = 1.f, m2 = 0.f, r2 = 1.f;
     if constexpr (POST) {
-      stats<EPT, VEC>(x, c0, step, a.D, a.rms, a.eps, sum, m1, r1);
+      stats<VEC, NC, PLACE>(x, col, a.D, a.rms, a.eps, sum, m1, r1);
+      w1.get(col, w);
+      b1.get(col, bb);
 #pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const int c = c0 + i * step, n = a.D - c;
-        float w[VEC], bb[VEC];
-        load_param<T, VEC>(a.post_scale, a.param32, c, n, 1.f, w);
-        load_param<T, VEC>(a.post_bias, a.param32, c, n, 0.f, bb);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v)
-          x[i * VEC + v] = (x[i * VEC + v] - m1) * r1 * w[v] + bb[v];
-      }
+      for (int e = 0; e < EPT; ++e) x[e] = (x[e] - m1) * r1 * w[e] + bb[e];
     }
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      float ca, cb, k, k1;
-      coefs<T, GATE>(a, GATE ? gt[i] : 0.f, ca, cb, k, k1);
-      const bool in = c0 + (i / VEC) * step + i % VEC < a.D;
-      s[i] = in ? ca * s[i] + cb * x[i] : 0.f;
+    for (int e = 0; e < EPT; ++e) {
+      float ca, cb, k1;
+      coefs<T, GATE>(a.alpha, gt[e], ca, cb, k1);
+      s[e] = ca * s[e] + cb * x[e];
     }
     if (on) {
 #pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const int c = c0 + i * step;
-        store_f32<T, VEC>((T*)a.s + base + c, a.D - c, s + i * VEC);
-      }
+      for (int i = 0; i < NC; ++i)
+        if (col.any(i, a.D))
+          store_vec<T, VEC>((T*)a.s + base + col.at[i], s + i * VEC);
     }
     if constexpr (PRE) {
-      stats<EPT, VEC>(s, c0, step, a.D, a.rms, a.eps, sum, m2, r2);
+      stats<VEC, NC, PLACE>(s, col, a.D, a.rms, a.eps, sum, m2, r2);
+      w2.get(col, w);
+      b2.get(col, bb);
 #pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const int c = c0 + i * step, n = a.D - c;
-        float w[VEC], bb[VEC];
-        load_param<T, VEC>(a.pre_scale, a.param32, c, n, 1.f, w);
-        load_param<T, VEC>(a.pre_bias, a.param32, c, n, 0.f, bb);
+      for (int e = 0; e < EPT; ++e) s[e] = (s[e] - m2) * r2 * w[e] + bb[e];
+      if (on) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v)
-          s[i * VEC + v] = (s[i * VEC + v] - m2) * r2 * w[v] + bb[v];
-        if (on) store_f32<T, VEC>((T*)a.h + base + c, n, s + i * VEC);
+        for (int i = 0; i < NC; ++i)
+          if (col.any(i, a.D))
+            store_vec<T, VEC>((T*)a.h + base + col.at[i], s + i * VEC);
       }
     }
-    if (a.stat && on && lane == 0) {
+    if (a.stat && on && it.lane == 0) {
       a.stat[row] = m1;
       a.stat[a.rows + row] = r1;
       a.stat[2 * a.rows + row] = m2;
@@ -258,179 +392,172 @@ __global__ __launch_bounds__(MAXT) void join_fwd_kernel(NormArgs a) {
   }
 }
 
-template <typename T, int EPT, bool POST, bool PRE, int GATE, int MAXT>
+template <typename T, int VEC, int EPT, int PLACE, bool POST, bool PRE,
+          int GATE, int MAXT>
 __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
-  constexpr int VEC = vec_of<T>(), NC = EPT / VEC;
+  constexpr int NC = EPT / VEC;
+  // blocks of 1024 have 128 registers a lane: parameters are read again for
+  // each row and nothing is fetched ahead
+  constexpr bool KEEP = MAXT <= 512;
+  using Raw = RawRow<T, VEC, NC>;
   __shared__ float buf[2][32];
-  __shared__ float fold[EPT * 256];  // the groups' sums of one parameter
-  RowSum sum(buf, a.tpr);
-  const int lane = threadIdx.x & (a.tpr - 1);
-  const int rpb = max((int)blockDim.x / a.tpr, 1);
-  const int c0 = lane * VEC, step = a.tpr * VEC;
+  // the lane groups' sums of one parameter
+  __shared__ float fold[PLACE == kBlock ? 1 : EPT * 256];
+  RowSum<PLACE> sum(buf, a.tpr);
+  const Rows<PLACE> it(a);
+  const Columns<VEC, NC> col(it.lane, a.tpr, a.D);
+  const Param<T, VEC, NC, KEEP> w1(POST ? a.post_scale : nullptr, a.param32, 1.f,
+                             col);
+  const Param<T, VEC, NC, KEEP> b1(POST ? a.post_bias : nullptr, a.param32, 0.f,
+                             col);
+  const Param<T, VEC, NC, KEEP> w2(PRE ? a.pre_scale : nullptr, a.param32, 1.f, col);
+  const Param<T, VEC, NC, KEEP> gp(is_channel(GATE) ? a.gate : nullptr,
+                             a.param32, 0.f, col);
+  // s and u are needed by the next norm and by the gate
+  constexpr bool NEED = PRE || GATE != kNone;
 
-  float acc[kNumParams][EPT];  // the unused ones are optimised out
+  float acc[kNumSums][EPT];  // the unused ones are optimised out
 #pragma unroll
-  for (int p = 0; p < kNumParams; ++p)
+  for (int p = 0; p < kNumSums; ++p)
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) acc[p][i] = 0.f;
+    for (int e = 0; e < EPT; ++e) acc[p][e] = 0.f;
 
-  for (long r0 = (long)blockIdx.x * rpb; r0 < a.rows;
-       r0 += (long)gridDim.x * rpb) {
-    long row = r0 + threadIdx.x / a.tpr;
-    const bool on = row < a.rows;
-    if (!on) row = a.rows - 1;
+  Raw xr, rr, dr, hr, gr;
+  float st[4];
+  auto fetch = [&](long row) __attribute__((always_inline)) {
+    row = min(row, a.rows - 1);
     const long base = row * a.D;
-    float x[EPT], rs[EPT], ds[EPT], dh[EPT], gt[EPT];
+    if constexpr (POST || NEED) xr.load((const T*)a.x + base, col);
+    if constexpr (NEED) rr.load((const T*)a.res + base, col);
+    dr.zero();
+    hr.zero();
+    if (a.dsum) dr.load((const T*)a.dsum + base, col);
+    if (PRE && a.dh) hr.load((const T*)a.dh + base, col);
+    if constexpr (is_token(GATE)) gr.load((const T*)a.gate + base, col);
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int c = c0 + i * step, n = a.D - c;
-      if constexpr (POST || PRE || GATE != kGateNone)
-        load_f32<T, VEC>((const T*)a.x + base + c, n, x + i * VEC);
-      if constexpr (PRE || GATE != kGateNone)
-        load_f32<T, VEC>((const T*)a.res + base + c, n, rs + i * VEC);
-      if (a.dsum) {
-        load_f32<T, VEC>((const T*)a.dsum + base + c, n, ds + i * VEC);
-      } else {
+    for (int i = 0; i < 4; ++i) st[i] = a.stat[i * a.rows + row];
+  };
+  if (KEEP) fetch(it.row);
+  for (long r0 = 0, n = (a.rows + it.stride - 1) / it.stride; r0 < n; ++r0) {
+    const long row = it.row + r0 * it.stride;
+    if (PLACE != kPartWave && row >= a.rows) break;
+    if (!KEEP) fetch(row);
+    const bool on = row < a.rows;
+    const long base = row * a.D;
+    // this row, 16-bit values kept as they are until they are used
+    const Raw rc = rr, dc = dr, hc = hr, gc = gr;
+    const float m1 = st[0], r1 = st[1], m2 = st[2], r2 = st[3];
+    float x[EPT], ds[EPT], w[EPT], bb[EPT], gt[EPT];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) ds[i * VEC + v] = 0.f;
+    for (int e = 0; e < EPT; ++e)  // the normalised row
+      x[e] = POST ? (xr[e] - m1) * r1 : NEED ? xr[e] : 0.f;
+    if (KEEP && r0 + 1 < n) fetch(row + it.stride);
+    auto gates = [&]() __attribute__((always_inline)) {
+      if constexpr (is_channel(GATE)) gp.get(col, gt);
+#pragma unroll
+      for (int e = 0; e < EPT; ++e)
+        if constexpr (!is_channel(GATE)) gt[e] = is_token(GATE) ? gc[e] : 0.f;
+    };
+    if constexpr (PRE) {
+      float sh[EPT], gh[EPT], p = 0.f, q = 0.f;
+      if constexpr (POST) w1.get(col, w), b1.get(col, bb);
+      gates();
+#pragma unroll
+      for (int e = 0; e < EPT; ++e) {
+        float ca, cb, k1;
+        coefs<T, GATE>(a.alpha, gt[e], ca, cb, k1);
+        const float u = POST ? x[e] * w[e] + bb[e] : x[e];
+        sh[e] = (ca * rc[e] + cb * u - m2) * r2;
       }
-      if constexpr (PRE) {
-        if (a.dh) {
-          load_f32<T, VEC>((const T*)a.dh + base + c, n, dh + i * VEC);
-        } else {
+      w2.get(col, w);
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) dh[i * VEC + v] = 0.f;
-        }
+      for (int e = 0; e < EPT; ++e) {
+        const float g = on ? hc[e] : 0.f;  // no row, no part in the sums
+        acc[kP1][e] += on ? g * sh[e] : 0.f;
+        acc[kP0][e] += g;
+        gh[e] = g * w[e];
+        p += col.own(e) ? gh[e] : 0.f;
+        q += col.own(e) ? gh[e] * sh[e] : 0.f;
       }
-    }
-    if constexpr (GATE != kGateNone)
-      load_gate<T, EPT, GATE>(a, row, c0, step, gt);
-    const float m1 = a.stat[row], r1 = a.stat[a.rows + row];
-    const float m2 = a.stat[2 * a.rows + row], r2 = a.stat[3 * a.rows + row];
-    if (!on) {  // nothing may reach the parameter sums
+      sum(p, q);
+      p = a.rms ? 0.f : p / a.D;
+      q /= a.D;
 #pragma unroll
-      for (int i = 0; i < EPT; ++i) ds[i] = dh[i] = 0.f;
-    }
-    // x becomes the normalised row
-    float u[EPT];
-    if constexpr (POST) {
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const int c = c0 + i * step, n = a.D - c;
-        float w[VEC], bb[VEC];
-        load_param<T, VEC>(a.post_scale, a.param32, c, n, 1.f, w);
-        load_param<T, VEC>(a.post_bias, a.param32, c, n, 0.f, bb);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          const int e = i * VEC + v;
-          x[e] = (x[e] - m1) * r1;
-          u[e] = x[e] * w[v] + bb[v];
-        }
-      }
+      for (int e = 0; e < EPT; ++e)
+        ds[e] = (on ? dc[e] : 0.f) + r2 * (gh[e] - p - sh[e] * q);
     } else {
 #pragma unroll
-      for (int i = 0; i < EPT; ++i) u[i] = x[i];
+      for (int e = 0; e < EPT; ++e) ds[e] = on ? dc[e] : 0.f;
     }
-    if constexpr (PRE) {
-      float sh[EPT], p = 0.f, q = 0.f;
+    float p = 0.f, q = 0.f, dr_[EPT];
+    gates();
+    if constexpr (POST) w1.get(col, w);
+    if constexpr (POST && is_token(GATE)) b1.get(col, bb);
 #pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const int c = c0 + i * step;
-        float w[VEC];
-        load_param<T, VEC>(a.pre_scale, a.param32, c, a.D - c, 1.f, w);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          const int e = i * VEC + v;
-          float ca, cb, k, k1;
-          coefs<T, GATE>(a, GATE ? gt[e] : 0.f, ca, cb, k, k1);
-          sh[e] = (ca * rs[e] + cb * u[e] - m2) * r2;
-          acc[kPreScale][e] += dh[e] * sh[e];
-          acc[kPreBias][e] += dh[e];
-          dh[e] *= w[v];  // 0 where there is no element
-          p += dh[e];
-          q += dh[e] * sh[e];
-        }
+    for (int e = 0; e < EPT; ++e) {
+      float ca, cb, k1;
+      coefs<T, GATE>(a.alpha, gt[e], ca, cb, k1);
+      const float d = ds[e];
+      dr_[e] = ca * d;   // the gradient of res
+      ds[e] = cb * d;    // and of u
+      if constexpr (is_channel(GATE) || POST) {
+        const float t = is_channel(GATE) ? d : ds[e];
+        acc[kS1][e] += on ? t * x[e] : 0.f;
+        acc[kS0][e] += on ? t : 0.f;
+        if constexpr (GATE == kHighCh) acc[kS2][e] += on ? d * rc[e] : 0.f;
       }
-      sum(p, q);
-      p = a.rms ? 0.f : p / a.D;
-      q /= a.D;
-#pragma unroll
-      for (int i = 0; i < EPT; ++i) ds[i] += r2 * (dh[i] - p - sh[i] * q);
-    }
-    float p = 0.f, q = 0.f, du[EPT];
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int c = c0 + i * step, n = a.D - c;
-      float w[VEC], dr[VEC], dg[VEC];
-      if constexpr (POST)
-        load_param<T, VEC>(a.post_scale, a.param32, c, n, 1.f, w);
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        const int e = i * VEC + v;
-        float ca, cb, k, k1;
-        coefs<T, GATE>(a, GATE ? gt[e] : 0.f, ca, cb, k, k1);
-        const float d = c + v < a.D ? ds[e] : 0.f;
-        dr[v] = ca * d;
-        du[e] = cb * d;
-        if constexpr (GATE != kGateNone) {
-          dg[v] = (a.highway ? k * k1 * (u[e] - a.alpha * rs[e]) : u[e]) * d;
-          // a row of another lane group's past the end adds nothing
-          if (!on) dg[v] = 0.f;
-          if constexpr (GATE == kGateChannel) acc[kGate][e] += dg[v];
-        }
-        if constexpr (POST) {
-          acc[kPostScale][e] += on ? du[e] * x[e] : 0.f;
-          acc[kPostBias][e] += on ? du[e] : 0.f;
-          du[e] *= w[v];
-          p += du[e];
-          q += du[e] * x[e];
-        }
+      if constexpr (is_token(GATE)) {
+        const float u = POST ? x[e] * w[e] + bb[e] : x[e];
+        gt[e] = (is_highway(GATE) ? cb * k1 * (u - a.alpha * rc[e]) : u) * d;
       }
-      if (on && a.dres) store_f32<T, VEC>((T*)a.dres + base + c, n, dr);
-      if constexpr (GATE == kGateToken)
-        if (on && a.dgate) store_f32<T, VEC>((T*)a.dgate + base + c, n, dg);
+      if constexpr (POST) {
+        ds[e] *= w[e];
+        p += col.own(e) ? ds[e] : 0.f;
+        q += col.own(e) ? ds[e] * x[e] : 0.f;
+      }
     }
+    auto put = [&](void* out, const float* v) __attribute__((always_inline)) {
+      if (!on || !out) return;
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (col.any(i, a.D))
+          store_vec<T, VEC>((T*)out + base + col.at[i], v + i * VEC);
+    };
+    put(a.dres, dr_);
+    if constexpr (is_token(GATE)) put(a.dgate, gt);
     if constexpr (POST) {
       sum(p, q);
       p = a.rms ? 0.f : p / a.D;
       q /= a.D;
 #pragma unroll
-      for (int i = 0; i < EPT; ++i) du[i] = r1 * (du[i] - p - x[i] * q);
+      for (int e = 0; e < EPT; ++e) ds[e] = r1 * (ds[e] - p - x[e] * q);
     }
-    if (on && a.dx) {
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const int c = c0 + i * step;
-        store_f32<T, VEC>((T*)a.dx + base + c, a.D - c, du + i * VEC);
-      }
-    }
+    put(a.dx, ds);
   }
   if (!a.part) return;
   float* part = a.part + (size_t)blockIdx.x * a.n_part * a.D;
 #pragma unroll
-  for (int p = 0; p < kNumParams; ++p) {
+  for (int p = 0; p < kNumSums; ++p) {
     if (a.slot[p] < 0) continue;
     float* out = part + (size_t)a.slot[p] * a.D;
-    if (rpb == 1) {
+    if constexpr (PLACE == kBlock) {
 #pragma unroll
-      for (int i = 0; i < EPT; ++i) {
-        const int c = c0 + (i / VEC) * step + i % VEC;
-        if (c < a.D) out[c] = acc[p][i];
-      }
+      for (int e = 0; e < EPT; ++e)
+        if (col.own(e)) out[col.at[e / VEC] + e % VEC] = acc[p][e];
     } else {  // blockDim.x is 256 here
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < EPT; ++i)
-        fold[i * 256 + threadIdx.x] = acc[p][i];
+      for (int e = 0; e < EPT; ++e)
+        fold[e * 256 + threadIdx.x] = acc[p][e];
       __syncthreads();
       if (threadIdx.x < a.tpr) {
+        const int groups = 256 / a.tpr;
 #pragma unroll
-        for (int i = 0; i < EPT; ++i) {
-          const int c = c0 + (i / VEC) * step + i % VEC;
+        for (int e = 0; e < EPT; ++e) {
           float t = 0.f;
-          for (int g = 0; g < rpb; ++g)
-            t += fold[i * 256 + g * a.tpr + threadIdx.x];
-          if (c < a.D) out[c] = t;
+          for (int g = 0; g < groups; ++g)
+            t += fold[e * 256 + g * a.tpr + threadIdx.x];
+          if (col.own(e)) out[col.at[e / VEC] + e % VEC] = t;
         }
       }
     }
@@ -439,42 +566,84 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
 
 struct NormPlan {
   NormArgs a{};
-  int gate_mode = kGateNone;
-  int ept = 8, threads = 256, rpb = 1;
+  int gate = kNone;
+  int ept = 8, place = kWave, threads = 256, rpb = 1;
 };
 
-#define GATES(T, EPT, POST, PRE, MAXT, FN)                              \
-  if (pl.gate_mode == kGateNone) { FN(T, EPT, POST, PRE, kGateNone, MAXT); }      \
-  else if (pl.gate_mode == kGateChannel) { FN(T, EPT, POST, PRE, kGateChannel, MAXT); } \
-  else { FN(T, EPT, POST, PRE, kGateToken, MAXT); }
-#define SIDES(T, EPT, MAXT, FN)                                         \
-  if (a.post_scale && a.pre_scale) { GATES(T, EPT, true, true, MAXT, FN) }        \
-  else if (a.post_scale) { GATES(T, EPT, true, false, MAXT, FN) }       \
-  else if (a.pre_scale) { GATES(T, EPT, false, true, MAXT, FN) }        \
-  else { GATES(T, EPT, false, false, MAXT, FN) }
-#define WIDTHS(T, FN)                                                   \
-  if (pl.ept == 8) { SIDES(T, 8, 512, FN) }                             \
-  else if (pl.threads <= 512) { SIDES(T, 16, 512, FN) }                 \
-  else { SIDES(T, 16, 1024, FN) }
+#define GATES(T, VEC, EPT, PLACE, POST, PRE, MAXT, FN)                    \
+  switch (pl.gate) {                                                      \
+    case kNone: FN(T, VEC, EPT, PLACE, POST, PRE, kNone, MAXT) break;     \
+    case kScaleCh: FN(T, VEC, EPT, PLACE, POST, PRE, kScaleCh, MAXT) break;   \
+    case kScaleTok: FN(T, VEC, EPT, PLACE, POST, PRE, kScaleTok, MAXT) break;  \
+    case kHighCh: FN(T, VEC, EPT, PLACE, POST, PRE, kHighCh, MAXT) break;     \
+    default: FN(T, VEC, EPT, PLACE, POST, PRE, kHighTok, MAXT)            \
+  }
+#define SIDES(T, VEC, EPT, PLACE, MAXT, FN)                               \
+  if (a.post_scale && a.pre_scale) {                                      \
+    GATES(T, VEC, EPT, PLACE, true, true, MAXT, FN)                       \
+  } else if (a.post_scale) {                                              \
+    GATES(T, VEC, EPT, PLACE, true, false, MAXT, FN)                      \
+  } else if (a.pre_scale) {                                               \
+    GATES(T, VEC, EPT, PLACE, false, true, MAXT, FN)                      \
+  } else {                                                                \
+    GATES(T, VEC, EPT, PLACE, false, false, MAXT, FN)                     \
+  }
+#define WIDTHS(T, FN)                                                     \
+  constexpr int V = 16 / (int)sizeof(T);                                  \
+  if (pl.ept == 1) { SIDES(T, 1, 1, kPartWave, 256, FN) }                 \
+  else if (pl.place == kPartWave) { SIDES(T, V, 8, kPartWave, 256, FN) }  \
+  else if (pl.place == kWave && pl.ept == 8) {                            \
+    SIDES(T, V, 8, kWave, 256, FN)                                        \
+  } else if (pl.place == kWave) { SIDES(T, V, 16, kWave, 256, FN) }       \
+  else if (pl.ept == 8) { SIDES(T, V, 8, kBlock, 512, FN) }               \
+  else if (pl.threads <= 512) { SIDES(T, V, 16, kBlock, 512, FN) }        \
+  else { SIDES(T, V, 16, kBlock, 1024, FN) }
 
+// blocks of a kernel that a CU holds at once, asked for once per block size
+template <auto KERNEL>
+int resident(int threads) {
+  static std::atomic<int> known[11];  // by log2(threads)
+  std::atomic<int>& k = known[__builtin_ctz((unsigned)threads)];
+  int n = k.load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(
+            &n, reinterpret_cast<const void*>(KERNEL), threads, 0) !=
+            hipSuccess || n < 1)
+      n = 1;
+    k.store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+// grid == 0: nothing is launched, the blocks that a CU holds are returned
 template <typename T>
-void join_fwd_launch(const NormPlan& pl, unsigned grid, hipStream_t stream) {
+int join_fwd_launch(const NormPlan& pl, unsigned grid, hipStream_t stream) {
   const NormArgs& a = pl.a;
-#define RUN(T, EPT, POST, PRE, GATE, MAXT)                                   \
-  hipLaunchKernelGGL((join_fwd_kernel<T, EPT, POST, PRE, GATE, MAXT>),       \
-                     dim3(grid), dim3(pl.threads), 0, stream, a)
+#define RUN(T, VEC, EPT, PLACE, POST, PRE, GATE, MAXT)                       \
+  {                                                                          \
+    constexpr auto kernel =                                                  \
+        &join_fwd_kernel<T, VEC, EPT, PLACE, POST, PRE, GATE, MAXT>;         \
+    if (grid == 0) return resident<kernel>(pl.threads);                      \
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(pl.threads), 0, stream, a);  \
+  }
   WIDTHS(T, RUN)
 #undef RUN
+  return 0;
 }
 
 template <typename T>
-void join_bwd_launch(const NormPlan& pl, unsigned grid, hipStream_t stream) {
+int join_bwd_launch(const NormPlan& pl, unsigned grid, hipStream_t stream) {
   const NormArgs& a = pl.a;
-#define RUN(T, EPT, POST, PRE, GATE, MAXT)                                   \
-  hipLaunchKernelGGL((join_bwd_kernel<T, EPT, POST, PRE, GATE, MAXT>),       \
-                     dim3(grid), dim3(pl.threads), 0, stream, a)
+#define RUN(T, VEC, EPT, PLACE, POST, PRE, GATE, MAXT)                       \
+  {                                                                          \
+    constexpr auto kernel =                                                  \
+        &join_bwd_kernel<T, VEC, EPT, PLACE, POST, PRE, GATE, MAXT>;         \
+    if (grid == 0) return resident<kernel>(pl.threads);                      \
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(pl.threads), 0, stream, a);  \
+  }
   WIDTHS(T, RUN)
 #undef RUN
+  return 0;
 }
 
 #undef WIDTHS

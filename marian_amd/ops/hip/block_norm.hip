@@ -8,56 +8,86 @@
 using namespace mamd;
 
 namespace mamd {
-extern template void join_fwd_launch<bf16_t>(const NormPlan&, unsigned,
-                                             hipStream_t);
-extern template void join_fwd_launch<f16_t>(const NormPlan&, unsigned,
+extern template int join_fwd_launch<bf16_t>(const NormPlan&, unsigned,
                                             hipStream_t);
-extern template void join_fwd_launch<float>(const NormPlan&, unsigned,
+extern template int join_fwd_launch<f16_t>(const NormPlan&, unsigned,
                                             hipStream_t);
-extern template void join_bwd_launch<bf16_t>(const NormPlan&, unsigned,
-                                             hipStream_t);
-extern template void join_bwd_launch<f16_t>(const NormPlan&, unsigned,
+extern template int join_fwd_launch<float>(const NormPlan&, unsigned,
                                             hipStream_t);
-extern template void join_bwd_launch<float>(const NormPlan&, unsigned,
+extern template int join_bwd_launch<bf16_t>(const NormPlan&, unsigned,
+                                            hipStream_t);
+extern template int join_bwd_launch<f16_t>(const NormPlan&, unsigned,
+                                            hipStream_t);
+extern template int join_bwd_launch<float>(const NormPlan&, unsigned,
                                             hipStream_t);
 }  // namespace mamd
-
-#define NORM_DTYPES(st, FN)                                             \
-  if (st == torch::kBFloat16) FN<bf16_t>(pl, grid, stream);             \
-  else if (st == torch::kHalf) FN<f16_t>(pl, grid, stream);             \
-  else if (st == torch::kFloat32) FN<float>(pl, grid, stream);          \
-  else TORCH_CHECK(false, "block_norm: unsupported dtype");
 
 namespace {
 
 struct SumArgs {
   const float* part;
-  int n, n_part, D;
-  void* out[kNumParams];
+  int n, D;
+  int slot[kNumSums];
+  int gate;                  // kNone unless the gate is per channel
+  float alpha;
+  const void* gate_p;        // parameters as in NormArgs
+  const void* w1;
+  const void* b1;
+  void* out[kNumSums];       // dgate, dpost_scale, .._bias, dpre_scale, .._bias
 };
 
-// the blocks' partial sums: 64 columns per block, its 16 waves take every
-// 16th row and meet in LDS, always in the same order
-template <typename P>
+// The blocks' partial sums, and the parameter gradients from them: 16 columns
+// per block, its 64 lane groups take every 64th row and meet in LDS, always in
+// the same order.
+template <typename P, int NP>
 __global__ __launch_bounds__(1024) void param_sum_kernel(SumArgs a) {
-  __shared__ float buf[16][64];
-  const int lane = threadIdx.x & 63, wid = threadIdx.x / 64;
-  const int cols = (a.D + 63) / 64;
-  const int p = blockIdx.x / cols, c = (blockIdx.x % cols) * 64 + lane;
-  float t = 0.f;
+  __shared__ float buf[NP][64][17];
+  __shared__ float total[NP][16];
+  const int lane = threadIdx.x & 15, grp = threadIdx.x / 16;
+  const int c = blockIdx.x * 16 + lane;
+  float t[NP] = {};
   if (c < a.D) {
 #pragma unroll 4
-    for (int i = wid; i < a.n; i += 16)
-      t += a.part[((size_t)i * a.n_part + p) * a.D + c];
-  }
-  buf[wid][lane] = t;
-  __syncthreads();
-  if (wid == 0 && c < a.D) {
-    t = 0.f;
+    for (int i = grp; i < a.n; i += 64) {
+      const float* row = a.part + (size_t)i * NP * a.D + c;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t += buf[i][lane];
-    ((P*)a.out[p])[c] = (P)t;
+      for (int p = 0; p < NP; ++p) t[p] += row[(size_t)p * a.D];
+    }
   }
+#pragma unroll
+  for (int p = 0; p < NP; ++p) buf[p][grp][lane] = t[p];
+  __syncthreads();
+  if (grp < NP) {  // group p adds up the p-th sum
+    float v = 0.f;
+#pragma unroll 16
+    for (int i = 0; i < 64; ++i) v += buf[grp][i][lane];
+    total[grp][lane] = v;
+  }
+  __syncthreads();
+  if (grp != 0 || c >= a.D) return;
+  float sum[kNumSums];
+#pragma unroll
+  for (int p = 0; p < kNumSums; ++p)
+    sum[p] = a.slot[p] >= 0 ? total[a.slot[p]][lane] : 0.f;
+  const float s1 = sum[kS1], s0 = sum[kS0];
+  const float w1 = a.w1 ? (float)((const P*)a.w1)[c] : 1.f;
+  const float b1 = a.b1 ? (float)((const P*)a.b1)[c] : 0.f;
+  float b = 1.f, dg = 0.f;
+  if (a.gate != kNone) {
+    const float g = (float)((const P*)a.gate_p)[c];
+    dg = w1 * s1 + b1 * s0;
+    if (a.gate == kHighCh) {
+      float k1;
+      sigmoid2<float>(g, b, k1);
+      dg = b * k1 * (dg - a.alpha * sum[kS2]);
+    } else {
+      b = g;
+    }
+  }
+  const float o[kNumSums] = {dg, b * s1, b * s0, sum[kP1], sum[kP0]};
+#pragma unroll
+  for (int p = 0; p < kNumSums; ++p)
+    if (a.out[p]) ((P*)a.out[p])[c] = (P)o[p];
 }
 
 const void* param_ptr(const c10::optional<torch::Tensor>& p,
@@ -90,7 +120,7 @@ NormPlan make_plan(const torch::Tensor& x, const torch::Tensor& res,
                const c10::optional<torch::Tensor>& post_bias,
                const c10::optional<torch::Tensor>& pre_scale,
                const c10::optional<torch::Tensor>& pre_bias, bool rms,
-               double eps) {
+               double eps, bool bwd) {
   NormPlan pl;
   NormArgs& a = pl.a;
   TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.is_contiguous(),
@@ -104,10 +134,10 @@ NormPlan make_plan(const torch::Tensor& x, const torch::Tensor& res,
   bool seen = false;
   if (gate.has_value()) {
     if (gate->dim() == 1) {
-      pl.gate_mode = kGateChannel;
+      pl.gate = highway ? kHighCh : kScaleCh;
       a.gate = param_ptr(gate, x, a.param32, seen, "gate");
     } else {
-      pl.gate_mode = kGateToken;
+      pl.gate = highway ? kHighTok : kScaleTok;
       check_like(*gate, x, "gate");
       a.gate = gate->data_ptr();
     }
@@ -116,17 +146,66 @@ NormPlan make_plan(const torch::Tensor& x, const torch::Tensor& res,
   a.post_bias = param_ptr(post_bias, x, a.param32, seen, "post_bias");
   a.pre_scale = param_ptr(pre_scale, x, a.param32, seen, "pre_scale");
   a.pre_bias = param_ptr(pre_bias, x, a.param32, seen, "pre_bias");
-  a.highway = highway;
   a.rms = rms;
   a.alpha = (float)alpha;
   a.eps = (float)eps;
-  // a row's lanes: 8 elements each up to 4096, 16 above
-  pl.ept = a.D <= 4096 ? 8 : 16;
+  // A row's lanes: part of a wave up to 256 columns, a wave of 8 elements a
+  // lane up to 512, then a block of 8 elements a lane, 16 from 4097 columns
+  // on. The forward pass takes one wave up to 1024 columns of 16 bits (16
+  // elements a lane, no barriers: 110 us at 65536 x 1024 where two waves take
+  // 130); the backward pass would need 291 registers for that.
+  const int vec = x.element_size() == 2 ? 8 : 4;
+  if (a.D < vec) {
+    pl.ept = 1;
+    pl.place = kPartWave;
+  } else if (a.D <= 256) {
+    pl.place = kPartWave;
+  } else if (a.D <= 512) {
+    pl.place = kWave;
+  } else if (a.D <= 1024 && vec == 8 && !bwd) {
+    pl.ept = 16;
+    pl.place = kWave;
+  } else {
+    pl.ept = a.D <= 4096 ? 8 : 16;
+    pl.place = kBlock;
+  }
   a.tpr = 1;
   while (a.tpr * pl.ept < a.D) a.tpr *= 2;
-  pl.threads = a.tpr > WAVE ? a.tpr : 256;
+  if (pl.place == kWave) a.tpr = WAVE;
+  pl.threads = pl.place == kBlock ? a.tpr : 256;
   pl.rpb = pl.threads / a.tpr;
   return pl;
+}
+
+int dispatch(bool bwd, const torch::Tensor& x, const NormPlan& pl,
+             unsigned grid) {
+  auto stream = at::cuda::getCurrentHIPStream();
+  int n = 0;
+  if (x.scalar_type() == torch::kBFloat16)
+    n = bwd ? join_bwd_launch<bf16_t>(pl, grid, stream)
+            : join_fwd_launch<bf16_t>(pl, grid, stream);
+  else if (x.scalar_type() == torch::kHalf)
+    n = bwd ? join_bwd_launch<f16_t>(pl, grid, stream)
+            : join_fwd_launch<f16_t>(pl, grid, stream);
+  else if (x.scalar_type() == torch::kFloat32)
+    n = bwd ? join_bwd_launch<float>(pl, grid, stream)
+            : join_fwd_launch<float>(pl, grid, stream);
+  else
+    TORCH_CHECK(false, "block_norm: unsupported dtype");
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+  return n;
+}
+
+// The blocks that the GPU holds at once, which walk over the rows: more would
+// run as a second, partly filled round (125 us for 110 at 65536 x 1024 bf16
+// forward without a gate), and the backward pass writes partial sums for each.
+unsigned grid_of(bool bwd, const torch::Tensor& x, const NormPlan& pl,
+                 int min_rows) {
+  const long all = (pl.a.rows + pl.rpb - 1) / pl.rpb;
+  const long cus = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  if (all <= cus) return (unsigned)all;
+  const long few = std::max((all + min_rows - 1) / min_rows, cus);
+  return (unsigned)std::min(few, cus * dispatch(bwd, x, pl, 0));
 }
 
 }  // namespace
@@ -140,7 +219,7 @@ std::vector<torch::Tensor> block_norm_fwd(
     c10::optional<torch::Tensor> pre_bias, bool rms, double eps,
     bool want_stat) {
   NormPlan pl = make_plan(x, res, gate, highway, alpha, post_scale, post_bias,
-                      pre_scale, pre_bias, rms, eps);
+                      pre_scale, pre_bias, rms, eps, false);
   NormArgs& a = pl.a;
   const c10::DeviceGuard guard(x.device());
   auto s = torch::empty_like(x);
@@ -151,11 +230,7 @@ std::vector<torch::Tensor> block_norm_fwd(
   a.s = s.data_ptr();
   a.h = h.data_ptr();
   a.stat = want_stat ? stat.data_ptr<float>() : nullptr;
-  const long blocks = (a.rows + pl.rpb - 1) / pl.rpb;
-  const unsigned grid = (unsigned)std::min<long>(blocks, 1L << 20);
-  auto stream = at::cuda::getCurrentHIPStream();
-  NORM_DTYPES(x.scalar_type(), join_fwd_launch)
-  C10_HIP_KERNEL_LAUNCH_CHECK();
+  dispatch(false, x, pl, grid_of(false, x, pl, 1));
   return {s, h, stat};
 }
 
@@ -170,7 +245,7 @@ std::vector<torch::Tensor> block_norm_bwd(
     torch::Tensor stat, c10::optional<torch::Tensor> dsum,
     c10::optional<torch::Tensor> dh, std::vector<bool> want) {
   NormPlan pl = make_plan(x, res, gate, highway, alpha, post_scale, post_bias,
-                      pre_scale, pre_bias, rms, eps);
+                      pre_scale, pre_bias, rms, eps, true);
   NormArgs& a = pl.a;
   TORCH_CHECK(want.size() == 7, "block_norm_bwd: want must have 7 entries");
   TORCH_CHECK(stat.device() == x.device() &&
@@ -194,49 +269,60 @@ std::vector<torch::Tensor> block_norm_bwd(
   std::vector<torch::Tensor> out(7, none);
   if (want[0]) out[0] = torch::empty_like(x), a.dx = out[0].data_ptr();
   if (want[1]) out[1] = torch::empty_like(x), a.dres = out[1].data_ptr();
-  if (want[2] && pl.gate_mode == kGateToken)
+  const bool channel = is_channel(pl.gate);
+  if (want[2] && is_token(pl.gate))
     out[2] = torch::empty_like(x), a.dgate = out[2].data_ptr();
   SumArgs sm{};
   auto popt = x.options().dtype(a.param32 ? torch::kFloat32 : x.scalar_type());
-  auto vec = [&](int param, int at, bool there) {
-    a.slot[param] = -1;
-    if (!want[at] || !there) return;
+  auto vec = [&](int at, bool there) {
+    if (!want[at] || !there) return false;
     out[at] = torch::empty({a.D}, popt);
-    sm.out[a.n_part] = out[at].data_ptr();
-    a.slot[param] = a.n_part++;
+    sm.out[at - 2] = out[at].data_ptr();
+    return true;
   };
-  vec(kGate, 2, pl.gate_mode == kGateChannel);
-  vec(kPostScale, 3, a.post_scale);
-  vec(kPostBias, 4, a.post_bias);
-  vec(kPreScale, 5, a.pre_scale);
-  vec(kPreBias, 6, a.pre_bias);
+  const bool dg = vec(2, channel), dw1 = vec(3, a.post_scale),
+             db1 = vec(4, a.post_bias), dw2 = vec(5, a.pre_scale),
+             db2 = vec(6, a.pre_bias);
+  const bool use[kNumSums] = {dw1 || dg, db1 || (dg && a.post_bias),
+                              dg && pl.gate == kHighCh, dw2, db2};
+  for (int p = 0; p < kNumSums; ++p)
+    sm.slot[p] = a.slot[p] = use[p] ? a.n_part++ : -1;
   if (a.rows == 0) {
     for (auto& t : out) t.zero_();
     return out;
   }
-  const long blocks = (a.rows + pl.rpb - 1) / pl.rpb;
-  const unsigned grid =
-      (unsigned)std::min<long>(blocks, a.n_part ? 1024 : 1L << 20);
+  // 4 turns at least for each block: one turn's partial sums are as many
+  // bytes as most of what it reads
+  const unsigned grid = grid_of(true, x, pl, a.n_part ? 4 : 1);
   torch::Tensor part;
   if (a.n_part) {
     part = torch::empty({(long)grid, a.n_part, a.D},
                         x.options().dtype(torch::kFloat32));
     a.part = part.data_ptr<float>();
   }
-  auto stream = at::cuda::getCurrentHIPStream();
-  NORM_DTYPES(x.scalar_type(), join_bwd_launch)
-  C10_HIP_KERNEL_LAUNCH_CHECK();
+  dispatch(true, x, pl, grid);
   if (a.n_part) {
     sm.part = a.part;
-    sm.n = grid, sm.n_part = a.n_part, sm.D = a.D;
-    const unsigned sgrid = (unsigned)(((a.D + 63) / 64) * a.n_part);
+    sm.n = grid, sm.D = a.D;
+    sm.gate = channel ? pl.gate : kNone;
+    sm.alpha = a.alpha;
+    sm.gate_p = a.gate, sm.w1 = a.post_scale, sm.b1 = a.post_bias;
+    const unsigned sgrid = (unsigned)((a.D + 15) / 16);
+    auto stream = at::cuda::getCurrentHIPStream();
+#define SUMN(P, NP)                                                          \
+  case NP:                                                                   \
+    hipLaunchKernelGGL((param_sum_kernel<P, NP>), dim3(sgrid), dim3(1024),   \
+                       0, stream, sm);                                       \
+    break;
 #define SUM(P)                                                               \
-  hipLaunchKernelGGL((param_sum_kernel<P>), dim3(sgrid), dim3(1024), 0,      \
-                     stream, sm)
-    if (a.param32 || x.scalar_type() == torch::kFloat32) { SUM(float); }
-    else if (x.scalar_type() == torch::kBFloat16) { SUM(bf16_t); }
-    else { SUM(f16_t); }
+  switch (a.n_part) {                                                        \
+    SUMN(P, 1) SUMN(P, 2) SUMN(P, 3) SUMN(P, 4) SUMN(P, 5)                   \
+  }
+    if (a.param32 || x.scalar_type() == torch::kFloat32) { SUM(float) }
+    else if (x.scalar_type() == torch::kBFloat16) { SUM(bf16_t) }
+    else { SUM(f16_t) }
 #undef SUM
+#undef SUMN
     C10_HIP_KERNEL_LAUNCH_CHECK();
   }
   return out;
