@@ -125,12 +125,14 @@ class ConfigParser:
         a("transformer-aan-nogate", "bool", False, "Omit AAN gate", "model")
         a("transformer-decoder-autoreg", str, "self-attention",
           "Autoregressive layer in decoder", "model",
-          choices=["self-attention", "average-attention"])
+          choices=["self-attention", "average-attention", "rnn"])
         a("transformer-tied-layers", int, [], "Tie encoder/decoder layers", "model", nargs="+")
         a("transformer-guided-alignment-layer", str, "last",
           "Decoder layer for guided alignment", "model")
-        a("transformer-preprocess", str, "", "Ops before each transformer block (d/a/n)", "model")
-        a("transformer-postprocess", str, "dan", "Ops after each transformer block (d/a/n)", "model")
+        a("transformer-preprocess", str, "", "Ops before each transformer block (d/a/n, r: RMS norm)", "model")
+        a("transformer-postprocess", str, "dan", "Ops after each transformer block (d/a/n, r: RMS norm, "
+          "g: learned gate per channel, h: highway with the residual)", "model")
+        a("transformer-residual-scale", float, 1.0, "Factor of the residual in a and h", "model")
         a("transformer-postprocess-emb", str, "d", "Ops after embeddings (d/a/n)", "model")
         a("transformer-postprocess-top", str, "", "Final ops after last block", "model")
         a("transformer-train-position-embeddings", "bool", False,

@@ -4,12 +4,14 @@ models/transformer.h LayerAttention/LayerFFN helpers).
 Conventions:
 - weights are stored marian-style as ``[in, out]`` (x @ W + b) so the .npz
   round-trips bit-for-bit with the reference format;
-- pre/postprocess strings 'd' (dropout), 'a' (residual add), 'n' (LayerNorm)
-  follow --transformer-preprocess/-postprocess.
+- pre/postprocess strings 'd' (dropout), 'a' (residual add), 'n' (LayerNorm),
+  'r' (RMS norm), 'g' (learned gate per channel) and 'h' (highway with the
+  residual) follow --transformer-preprocess/-postprocess.
 """
 from __future__ import annotations
 
 import math
+import re
 from typing import Optional
 
 import torch
@@ -49,6 +51,25 @@ class LayerNorm(nn.Module):
 
     def forward(self, x):
         return ops.layer_norm(x, self.scale, self.bias, self.eps)
+
+
+def _vec(v, x):
+    """A parameter vector as ops.block_norm takes it beside rows x: of their
+    type or float32."""
+    return v if v.dtype in (x.dtype, torch.float32) else v.to(x.dtype)
+
+
+class RMSNorm(nn.Module):
+    """x / sqrt(mean(x^2) + eps) * scale."""
+
+    def __init__(self, dim: int, eps: float = 1e-9):
+        super().__init__()
+        self.scale = nn.Parameter(torch.ones(dim))
+        self.eps = eps
+
+    def forward(self, x):
+        return ops.block_norm(x, None, post_scale=_vec(self.scale, x),
+                              norm="rms", eps=self.eps)[0]
 
 
 def sinusoidal_position_embeddings(length: int, dim: int, start: int = 0,
@@ -127,16 +148,93 @@ class Embedding(nn.Module):
 
 class PrePostProcessor(nn.Module):
     """Applies a marian pre/postprocess op string: 'd'ropout, 'a'dd residual,
-    'n'ormalize (ref: transformer.h preProcess/postProcess)."""
+    'n'ormalize (ref: transformer.h preProcess/postProcess), and
+    'r' RMS norm, 'g' multiply by a learned gate per channel, 'h' highway:
+    k x + (1 - k) residual with k = sigmoid(residual W + b).
+    res_scale multiplies the residual of 'a' and 'h'.
 
-    def __init__(self, ops_str: str, dim: int, dropout: float):
+    Strings with r, g, h or a residual scale run on the fused block join
+    (ops.block_norm); the others keep their own kernels."""
+
+    def __init__(self, ops_str: str, dim: int, dropout: float,
+                 res_scale: float = 1.0):
         super().__init__()
         self.ops_str = ops_str
         self.dropout = dropout
+        self.res_scale = float(res_scale)
         if "n" in ops_str:
             self.ln = LayerNorm(dim)
+        if "r" in ops_str:
+            self.rms = RMSNorm(dim)
+        if "g" in ops_str:
+            self.gate = nn.Parameter(torch.ones(dim))
+        if "h" in ops_str:
+            self.highway = Dense(dim, dim)
+        self.extended = bool(set(ops_str) & set("rgh")) \
+            or self.res_scale != 1.0
+        # dropout, norm, gate, join, norm: what one fused call computes
+        m = re.fullmatch(r"(d?)([nr]?)(g?)([ah])([nr]?)", ops_str)
+        self.parts = m.groups() if m else None
+
+    def norm_args(self, op: str, side: str, x) -> dict:
+        """ops.block_norm's arguments for the norm `op` on one side."""
+        if op == "n":
+            return {side + "_scale": _vec(self.ln.scale, x),
+                    side + "_bias": _vec(self.ln.bias, x)}
+        return {side + "_scale": _vec(self.rms.scale, x)} if op == "r" else {}
+
+    def _drop(self, x):
+        if self.dropout > 0 and self.training:
+            return torch.nn.functional.dropout(x, self.dropout, True)
+        return x
+
+    def _fused(self, x, residual, pre_op: str = "", pre=None):
+        """(joined, normed): this string's ops with pre's norm `pre_op`
+        behind them, or None where one fused call cannot compute them."""
+        if self.parts is None:
+            return None
+        drop, norm, gate, join, _ = self.parts
+        kinds = {op for op in (norm, pre_op) if op}
+        if len(kinds) > 1 or (gate and join == "h"):
+            return None
+        kw = {**self.norm_args(norm, "post", x),
+              **(pre.norm_args(pre_op, "pre", x) if pre_op else {})}
+        if gate:
+            kw["gate"] = _vec(self.gate, x)
+        elif join == "h":
+            kw.update(gate=self.highway(residual), gate_kind="highway")
+        return ops.block_norm(self._drop(x) if drop else x, residual,
+                              res_scale=self.res_scale,
+                              norm="rms" if kinds == {"r"} else "layer",
+                              eps=1e-9, **kw)
+
+    def _forward_extended(self, x, residual):
+        if residual is not None:
+            tail = self.parts[4] if self.parts else ""
+            out = self._fused(x, residual, tail, self)
+            if out is not None:
+                return out[1] if tail else out[0]
+        for op in self.ops_str:
+            if op == "d":
+                x = self._drop(x)
+            elif op == "n":
+                x = self.ln(x)
+            elif op == "r":
+                x = self.rms(x)
+            elif op == "g":
+                x = ops.block_norm(x, None, gate=_vec(self.gate, x))[0]
+            elif op in "ah" and residual is not None:
+                kw = {} if op == "a" else dict(gate=self.highway(residual),
+                                               gate_kind="highway")
+                x = ops.block_norm(x, residual, res_scale=self.res_scale,
+                                   **kw)[0]
+            elif op not in "ah":
+                raise ValueError(f"Unknown pre/postprocess op '{op}'")
+        return x
 
     def forward(self, x, residual=None):
+        if self.extended:
+            return self._forward_extended(x, residual)
         ops_str = self.ops_str
         # 'an' tail with no active dropout: fused residual-add + LN kernel
         if residual is not None and ops_str.endswith("an") \
@@ -160,6 +258,18 @@ class PrePostProcessor(nn.Module):
             else:
                 raise ValueError(f"Unknown pre/postprocess op '{op}'")
         return x
+
+
+def join_blocks(post: PrePostProcessor, pre: PrePostProcessor, x, residual):
+    """The end of one block and the start of the next: y = post(x, residual)
+    and pre(y). One fused call where one of them needs it and both fit."""
+    if (post.extended or pre.extended) and post.parts is not None \
+            and not post.parts[4] and pre.ops_str in ("n", "r"):
+        out = post._fused(x, residual, pre.ops_str, pre)
+        if out is not None:
+            return out
+    y = post(x, residual=residual)
+    return y, pre(y)
 
 
 class MultiHeadAttention(nn.Module):
@@ -390,3 +500,52 @@ class AverageAttention(nn.Module):
             cache[key] = cache[key] + y
             a = (cache[key] / (step + 1)).to(y.dtype)
         return self._combine(y, self._ffn(a))
+
+
+class SSRU(nn.Module):
+    """Recurrent decoder self-attention replacement
+    (--transformer-decoder-autoreg rnn with --dec-cell ssru; ref:
+    models/transformer.h DecoderLayerRNN, rnn/cells.h SSRU):
+
+        f = sigmoid(x Wf + bf);  c = f c + (1 - f) (x W);  h = relu(c)
+
+    W and Wf are one [d, 2d] parameter, so a layer is one GEMM and one scan
+    over the sequence (decoding: one step on a float32 state)."""
+
+    def __init__(self, dim: int):
+        super().__init__()
+        self.dim = dim
+        self.W_xg = nn.Parameter(torch.empty(dim, 2 * dim))
+        self.bf = nn.Parameter(torch.zeros(dim))
+        for i in range(2):
+            nn.init.xavier_uniform_(self.W_xg[:, i * dim:(i + 1) * dim])
+
+    # marian-named views of the fused parameter
+    def w_slice(self, i):
+        return self.W_xg[:, i * self.dim:(i + 1) * self.dim]
+
+    def project(self, x):
+        """[x W, x Wf + bf]; only the gate half has a bias."""
+        if torch.is_grad_enabled():
+            return ops.linear(x, self.W_xg,
+                              torch.nn.functional.pad(self.bf, (self.dim, 0)))
+        xg = ops.linear(x, self.W_xg)   # packed int8 weights stay cached
+        xg[..., self.dim:] += self.bf.to(xg.dtype)
+        return xg
+
+    def step(self, x, state, inplace: bool = False):
+        """x [N, d], state float32 [N, d] -> (h [N, d], new state)."""
+        xg = self.project(x)
+        return ops.gated_step(xg[:, :self.dim], xg[:, self.dim:], state,
+                              act="relu", inplace=inplace)
+
+    def forward(self, x, cache=None, cache_key: str = ""):
+        """x: [B, T, d] (training) or [B, 1, d] (decode with cache)."""
+        if cache is None:
+            return ops.gated_scan_xg(self.project(x), act="relu")[0]
+        key = cache_key + "_cell"
+        if key not in cache:
+            cache[key] = torch.zeros(x.shape[0], self.dim, device=x.device,
+                                     dtype=torch.float32)
+        h, cache[key] = self.step(x[:, 0], cache[key])
+        return h[:, None]

@@ -23,8 +23,8 @@ import torch
 import torch.nn as nn
 
 from ..common.options import Options
-from .layers import (Dense, Embedding, FFN, MultiHeadAttention, 
-                     PrePostProcessor)
+from .layers import (Dense, Embedding, FFN, MultiHeadAttention,
+                     PrePostProcessor, SSRU, join_blocks)
 
 NEG_INF = -1e9  # marian uses additive log-masks with large negative value
 
@@ -38,10 +38,13 @@ class EncoderLayer(nn.Module):
     def __init__(self, opt):
         super().__init__()
         d, drop = opt["dim-emb"], opt.get("transformer-dropout", 0.0)
+        alpha = opt.get("transformer-residual-scale", 1.0)
         self.pre_self = PrePostProcessor(opt["transformer-preprocess"], d, drop)
-        self.post_self = PrePostProcessor(opt["transformer-postprocess"], d, drop)
+        self.post_self = PrePostProcessor(opt["transformer-postprocess"], d, drop,
+                                          alpha)
         self.pre_ffn = PrePostProcessor(opt["transformer-preprocess"], d, drop)
-        self.post_ffn = PrePostProcessor(opt["transformer-postprocess"], d, drop)
+        self.post_ffn = PrePostProcessor(opt["transformer-postprocess"], d, drop,
+                                          alpha)
         self.self_attn = MultiHeadAttention(
             d, opt["transformer-heads"],
             opt.get("transformer-dropout-attention", 0.0),
@@ -54,8 +57,7 @@ class EncoderLayer(nn.Module):
     def forward(self, x, mask, lens=None):
         h = self.pre_self(x)
         h = self.self_attn(h, h, h, mask=mask, lens=lens)
-        x = self.post_self(h, residual=x)
-        h = self.pre_ffn(x)
+        x, h = join_blocks(self.post_self, self.pre_ffn, h, x)
         h = self.ffn(h)
         return self.post_ffn(h, residual=x)
 
@@ -64,13 +66,17 @@ class DecoderLayer(nn.Module):
     def __init__(self, opt):
         super().__init__()
         d, drop = opt["dim-emb"], opt.get("transformer-dropout", 0.0)
+        alpha = opt.get("transformer-residual-scale", 1.0)
         dim_ffn = opt.get("transformer-decoder-dim-ffn", 0) or opt["transformer-dim-ffn"]
         self.pre_self = PrePostProcessor(opt["transformer-preprocess"], d, drop)
-        self.post_self = PrePostProcessor(opt["transformer-postprocess"], d, drop)
+        self.post_self = PrePostProcessor(opt["transformer-postprocess"], d, drop,
+                                          alpha)
         self.pre_ctx = PrePostProcessor(opt["transformer-preprocess"], d, drop)
-        self.post_ctx = PrePostProcessor(opt["transformer-postprocess"], d, drop)
+        self.post_ctx = PrePostProcessor(opt["transformer-postprocess"], d, drop,
+                                          alpha)
         self.pre_ffn = PrePostProcessor(opt["transformer-preprocess"], d, drop)
-        self.post_ffn = PrePostProcessor(opt["transformer-postprocess"], d, drop)
+        self.post_ffn = PrePostProcessor(opt["transformer-postprocess"], d, drop,
+                                          alpha)
         self.autoreg = opt.get("transformer-decoder-autoreg", "self-attention")
         if self.autoreg == "average-attention":
             from .layers import AverageAttention
@@ -79,6 +85,12 @@ class DecoderLayer(nn.Module):
                 opt.get("transformer-aan-activation", "swish"),
                 opt.get("transformer-ffn-depth-aan", 2),
                 not opt.get("transformer-aan-nogate", False), drop)
+        elif self.autoreg == "rnn":
+            cell = opt.get("dec-cell", "ssru")
+            if cell != "ssru":
+                raise ValueError("--transformer-decoder-autoreg rnn supports "
+                                 f"--dec-cell ssru, got {cell}")
+            self.self_attn = SSRU(d)
         else:
             self.self_attn = MultiHeadAttention(
                 d, opt["transformer-heads"],
@@ -98,20 +110,20 @@ class DecoderLayer(nn.Module):
                 cache: Optional[dict] = None, layer_id: int = 0,
                 src_lens=None, collect: Optional[dict] = None):
         h = self.pre_self(x)
-        if self.autoreg == "average-attention":
+        if self.autoreg in ("average-attention", "rnn"):
             h = self.self_attn(h, cache=cache, cache_key=f"l{layer_id}_self")
         else:
             h = self.self_attn(h, h, h, causal=causal, cache=cache,
                                cache_key=f"l{layer_id}_self")
-        x = self.post_self(h, residual=x)
         if enc_out is not None:   # LM decoders have no cross-attention
-            h = self.pre_ctx(x)
+            x, h = join_blocks(self.post_self, self.pre_ctx, h, x)
             h = self.context_attn(h, enc_out, enc_out, mask=src_mask,
                                   cache=cache,
                                   cache_key=f"l{layer_id}_context",
                                   lens=src_lens, collect=collect)
-            x = self.post_ctx(h, residual=x)
-        h = self.pre_ffn(x)
+            x, h = join_blocks(self.post_ctx, self.pre_ffn, h, x)
+        else:
+            x, h = join_blocks(self.post_self, self.pre_ffn, h, x)
         h = self.ffn(h)
         return self.post_ffn(h, residual=x)
 
@@ -125,6 +137,13 @@ class TransformerModel(nn.Module):
         dims = options.list("dim-vocabs")
         self.src_vocab_size = int(dims[0])
         self.trg_vocab_size = int(dims[-1])
+        # gates and highways join a block with its residual
+        for key, no in (("preprocess", "gh"), ("postprocess-emb", "rgh"),
+                        ("postprocess-top", "gh")):
+            bad = set(options.get("transformer-" + key, "") or "") & set(no)
+            if bad:
+                raise ValueError(f"--transformer-{key} does not take "
+                                 f"'{''.join(sorted(bad))}'")
         d = options["dim-emb"]
         self.dim = d
         drop = options.get("transformer-dropout", 0.0)
@@ -203,9 +222,10 @@ class TransformerModel(nn.Module):
                     for m in (layer.self_attn.Wo, layer.ffn.W2):
                         m.W.mul_(li ** -0.5)
                 for li, layer in enumerate(self.decoder, start=1):
-                    for m in (layer.self_attn.Wo, layer.context_attn.Wo,
-                              layer.ffn.W2):
-                        m.W.mul_(li ** -0.5)
+                    for m in (getattr(layer.self_attn, "Wo", None),
+                              layer.context_attn.Wo, layer.ffn.W2):
+                        if m is not None:   # not every autoreg layer has Wo
+                            m.W.mul_(li ** -0.5)
 
     def _guided_layer(self) -> int:
         g = self.opt.get("transformer-guided-alignment-layer", "last")
@@ -287,7 +307,8 @@ class TransformerModel(nn.Module):
         # single gather; per-layer views are refreshed each step (the beam
         # search replaces the backing tensor on reorder)
         max_len = cache.get("max_len", 0)
-        if max_len:
+        if max_len and isinstance(self.decoder[0].self_attn,
+                                  MultiHeadAttention):
             L = len(self.decoder)
             if "self_kv" not in cache:
                 H = self.decoder[0].self_attn.heads
@@ -436,6 +457,25 @@ class TransformerModel(nn.Module):
         if self.out_b is not None:
             m["decoder_ff_logit_out_b"] = self.out_b
 
+        def post_items(prefix: str, post: PrePostProcessor):
+            if hasattr(post, "ln"):
+                m[prefix + "_ln_scale"] = post.ln.scale
+                m[prefix + "_ln_bias"] = post.ln.bias
+            if hasattr(post, "rms"):
+                m[prefix + "_rms_scale"] = post.rms.scale
+            if hasattr(post, "gate"):
+                m[prefix + "_gate"] = post.gate
+            if hasattr(post, "highway"):
+                m[prefix + "_highway_W"] = post.highway.W
+                m[prefix + "_highway_b"] = post.highway.b
+
+        def pre_items(prefix: str, pre: Optional[PrePostProcessor]):
+            if pre is not None and hasattr(pre, "ln"):
+                m[prefix + "_ln_scale_pre"] = pre.ln.scale
+                m[prefix + "_ln_bias_pre"] = pre.ln.bias
+            if pre is not None and hasattr(pre, "rms"):
+                m[prefix + "_rms_scale_pre"] = pre.rms.scale
+
         def attn(prefix: str, a: MultiHeadAttention, post: PrePostProcessor):
             # marian names are VIEWS into the fused [d,3d] QKV parameter
             m[prefix + "_Wq"] = a.w_slice(0)
@@ -447,28 +487,20 @@ class TransformerModel(nn.Module):
             if not getattr(a, "no_projection", False):
                 m[prefix + "_Wo"] = a.Wo.W
                 m[prefix + "_bo"] = a.Wo.b
-            if hasattr(post, "ln"):
-                m[prefix + "_Wo_ln_scale"] = post.ln.scale
-                m[prefix + "_Wo_ln_bias"] = post.ln.bias
+            post_items(prefix + "_Wo", post)
 
         def ffn(prefix: str, f: FFN, post: PrePostProcessor):
             for li, d in enumerate(f.Ws, start=1):
                 m[f"{prefix}_W{li}"] = d.W
                 m[f"{prefix}_b{li}"] = d.b
-            if hasattr(post, "ln"):
-                m[prefix + "_ffn_ln_scale"] = post.ln.scale
-                m[prefix + "_ffn_ln_bias"] = post.ln.bias
+            post_items(prefix + "_ffn", post)
 
         for i, layer in enumerate(self.encoder, start=1):
             attn(f"encoder_l{i}_self", layer.self_attn, layer.post_self)
             ffn(f"encoder_l{i}_ffn", layer.ffn, layer.post_ffn)
-            # prenorm LNs live in the preprocessors
-            if hasattr(layer.pre_self, "ln"):
-                m[f"encoder_l{i}_self_Wq_ln_scale_pre"] = layer.pre_self.ln.scale
-                m[f"encoder_l{i}_self_Wq_ln_bias_pre"] = layer.pre_self.ln.bias
-            if hasattr(layer.pre_ffn, "ln"):
-                m[f"encoder_l{i}_ffn_W1_ln_scale_pre"] = layer.pre_ffn.ln.scale
-                m[f"encoder_l{i}_ffn_W1_ln_bias_pre"] = layer.pre_ffn.ln.bias
+            # prenorms live in the preprocessors
+            pre_items(f"encoder_l{i}_self_Wq", layer.pre_self)
+            pre_items(f"encoder_l{i}_ffn_W1", layer.pre_ffn)
         for i, layer in enumerate(self.decoder, start=1):
             if layer.autoreg == "average-attention":
                 a = layer.self_attn
@@ -479,30 +511,26 @@ class TransformerModel(nn.Module):
                 if a.gated:
                     m[f"decoder_l{i}_aan_Wi"] = a.Wi.W
                     m[f"decoder_l{i}_aan_bi"] = a.Wi.b
-                if hasattr(layer.post_self, "ln"):
-                    m[f"decoder_l{i}_aan_ln_scale"] = layer.post_self.ln.scale
-                    m[f"decoder_l{i}_aan_ln_bias"] = layer.post_self.ln.bias
+                post_items(f"decoder_l{i}_aan", layer.post_self)
+            elif layer.autoreg == "rnn":
+                a = layer.self_attn
+                m[f"decoder_l{i}_rnn_W"] = a.w_slice(0)
+                m[f"decoder_l{i}_rnn_Wf"] = a.w_slice(1)
+                m[f"decoder_l{i}_rnn_bf"] = a.bf
+                post_items(f"decoder_l{i}_rnn_ffn", layer.post_self)
             else:
                 attn(f"decoder_l{i}_self", layer.self_attn, layer.post_self)
             if layer.context_attn is not None:   # absent in LMs
                 attn(f"decoder_l{i}_context", layer.context_attn,
                      layer.post_ctx)
             ffn(f"decoder_l{i}_ffn", layer.ffn, layer.post_ffn)
-            if hasattr(layer.pre_self, "ln"):
-                m[f"decoder_l{i}_self_Wq_ln_scale_pre"] = layer.pre_self.ln.scale
-                m[f"decoder_l{i}_self_Wq_ln_bias_pre"] = layer.pre_self.ln.bias
-            if layer.pre_ctx is not None and hasattr(layer.pre_ctx, "ln"):
-                m[f"decoder_l{i}_context_Wq_ln_scale_pre"] = layer.pre_ctx.ln.scale
-                m[f"decoder_l{i}_context_Wq_ln_bias_pre"] = layer.pre_ctx.ln.bias
-            if hasattr(layer.pre_ffn, "ln"):
-                m[f"decoder_l{i}_ffn_W1_ln_scale_pre"] = layer.pre_ffn.ln.scale
-                m[f"decoder_l{i}_ffn_W1_ln_bias_pre"] = layer.pre_ffn.ln.bias
-        if self.post_top_enc is not None and hasattr(self.post_top_enc, "ln"):
-            m["encoder_top_ln_scale"] = self.post_top_enc.ln.scale
-            m["encoder_top_ln_bias"] = self.post_top_enc.ln.bias
-        if self.post_top_dec is not None and hasattr(self.post_top_dec, "ln"):
-            m["decoder_top_ln_scale"] = self.post_top_dec.ln.scale
-            m["decoder_top_ln_bias"] = self.post_top_dec.ln.bias
+            pre_items(f"decoder_l{i}_self_Wq", layer.pre_self)
+            pre_items(f"decoder_l{i}_context_Wq", layer.pre_ctx)
+            pre_items(f"decoder_l{i}_ffn_W1", layer.pre_ffn)
+        if self.post_top_enc is not None:
+            post_items("encoder_top", self.post_top_enc)
+        if self.post_top_dec is not None:
+            post_items("decoder_top", self.post_top_dec)
         return m
 
     def marian_items(self) -> Dict[str, np.ndarray]:
@@ -545,6 +573,10 @@ class TransformerModel(nn.Module):
                 "transformer-train-position-embeddings",
                 "tied-embeddings", "tied-embeddings-src",
                 "tied-embeddings-all", "output-omit-bias"]
+        if self.opt.get("transformer-decoder-autoreg", "") == "rnn":
+            keys.append("dec-cell")
+        if self.opt.get("transformer-residual-scale", 1.0) != 1.0:
+            keys.append("transformer-residual-scale")
         cfg = {k: self.opt.get(k) for k in keys if self.opt.has(k)}
         cfg["version"] = "marian_amd v0.1.0"
         return cfg

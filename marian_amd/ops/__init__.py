@@ -241,7 +241,7 @@ def layer_norm_residual(x: torch.Tensor, res: torch.Tensor,
 # The join of two transformer blocks (ref: transformer.h pre/postProcess)
 # ---------------------------------------------------------------------------
 
-def block_norm(x: torch.Tensor, res: torch.Tensor,
+def block_norm(x: torch.Tensor, res: Optional[torch.Tensor],
                gate: Optional[torch.Tensor] = None, gate_kind: str = "scale",
                res_scale: float = 1.0,
                post_scale: Optional[torch.Tensor] = None,
@@ -260,7 +260,7 @@ def block_norm(x: torch.Tensor, res: torch.Tensor,
 
     norm: "layer" ((v - mean) / sqrt(var + eps)) or "rms" (v / sqrt(mean v^2
     + eps)), times scale, plus bias if there is one. x, res: [..., D], fp32 /
-    bf16 / fp16, D <= 16384. gate: [D] (per channel) or x's shape (per
+    bf16 / fp16, D <= 16384; without res its term is left out. gate: [D] (per channel) or x's shape (per
     token). Parameters are [D], all of x's dtype or all float32. h is taken
     from the 32-bit s; s and h are rounded once. Differentiable once in every
     tensor.

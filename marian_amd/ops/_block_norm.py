@@ -22,8 +22,8 @@ def check_join(x, res, gate, gate_kind, params, norm):
     if not 0 < D <= MAX_WIDTH:
         raise ValueError(f"block_norm: the width must be 1..{MAX_WIDTH}, "
                          f"got {D}")
-    if res.shape != x.shape or res.dtype != x.dtype \
-            or res.device != x.device:
+    if res is not None and (res.shape != x.shape or res.dtype != x.dtype
+                            or res.device != x.device):
         raise ValueError("block_norm: res must have x's shape, dtype and "
                          "device")
     if norm not in ("layer", "rms"):
@@ -32,6 +32,8 @@ def check_join(x, res, gate, gate_kind, params, norm):
     if gate_kind not in ("scale", "highway"):
         raise ValueError("block_norm: gate_kind must be scale or highway, "
                          f"got {gate_kind!r}")
+    if res is None and gate_kind == "highway":
+        raise ValueError("block_norm: a highway needs res")
     vecs = {k: v for k, v in params.items() if v is not None}
     if gate is not None:
         if gate.dim() == 1 and gate.shape == (D,) and x.dim() > 1:
@@ -67,7 +69,7 @@ def block_norm_torch(x, res, gate=None, gate_kind="scale", res_scale=1.0,
         v = v * scale.to(acc)
         return v if bias is None else v + bias.to(acc)
 
-    u, r = x.to(acc), res.to(acc) * res_scale
+    u, r = x.to(acc), 0.0 if res is None else res.to(acc) * res_scale
     if post_scale is not None:
         u = normed(u, post_scale, post_bias)
     if gate is None:

@@ -66,8 +66,8 @@ std::tuple<torch::Tensor, torch::Tensor> gated_step(
     torch::Tensor x, torch::Tensor gate, c10::optional<torch::Tensor> state,
     std::string act, bool inplace);
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> block_norm(
-    torch::Tensor x, torch::Tensor res, c10::optional<torch::Tensor> gate,
-    std::string gate_kind, double alpha,
+    torch::Tensor x, c10::optional<torch::Tensor> res,
+    c10::optional<torch::Tensor> gate, std::string gate_kind, double alpha,
     c10::optional<torch::Tensor> post_scale,
     c10::optional<torch::Tensor> post_bias,
     c10::optional<torch::Tensor> pre_scale,

@@ -53,7 +53,7 @@ enum { kS1 = 0, kS0, kS2, kP1, kP0, kNumSums };
 
 struct NormArgs {
   const void* x;
-  const void* res;
+  const void* res;           // null: zeros
   const void* gate;          // null, [D] or [R,D]
   const void* post_scale;    // parameters: [D] or null
   const void* post_bias;
@@ -330,9 +330,10 @@ __global__ __launch_bounds__(MAXT) void join_fwd_kernel(NormArgs a) {
   auto fetch = [&](long row) __attribute__((always_inline)) {
     const long base = min(row, a.rows - 1) * a.D;
     xr.load((const T*)a.x + base, col);
-    rr.load((const T*)a.res + base, col);
+    if (a.res) rr.load((const T*)a.res + base, col);
     if constexpr (is_token(GATE)) gr.load((const T*)a.gate + base, col);
   };
+  rr.zero();
   if (KEEP) fetch(it.row);
   // the same number of turns for all lanes of a wave
   for (long r0 = 0, n = (a.rows + it.stride - 1) / it.stride; r0 < n; ++r0) {
@@ -424,11 +425,12 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
 
   Raw xr, rr, dr, hr, gr;
   float st[4];
+  rr.zero();
   auto fetch = [&](long row) __attribute__((always_inline)) {
     row = min(row, a.rows - 1);
     const long base = row * a.D;
     if constexpr (POST || NEED) xr.load((const T*)a.x + base, col);
-    if constexpr (NEED) rr.load((const T*)a.res + base, col);
+    if (NEED && a.res) rr.load((const T*)a.res + base, col);
     dr.zero();
     hr.zero();
     if (a.dsum) dr.load((const T*)a.dsum + base, col);

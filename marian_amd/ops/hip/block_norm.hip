@@ -114,7 +114,8 @@ void check_like(const torch::Tensor& t, const torch::Tensor& x,
               "block_norm: ", what, " must be dense and like x");
 }
 
-NormPlan make_plan(const torch::Tensor& x, const torch::Tensor& res,
+NormPlan make_plan(const torch::Tensor& x,
+                   const c10::optional<torch::Tensor>& res,
                const c10::optional<torch::Tensor>& gate, bool highway,
                double alpha, const c10::optional<torch::Tensor>& post_scale,
                const c10::optional<torch::Tensor>& post_bias,
@@ -125,12 +126,12 @@ NormPlan make_plan(const torch::Tensor& x, const torch::Tensor& res,
   NormArgs& a = pl.a;
   TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.is_contiguous(),
               "block_norm: x must be dense [R, D] on a GPU");
-  check_like(res, x, "res");
+  if (res.has_value()) check_like(*res, x, "res");
   TORCH_CHECK(x.size(1) > 0 && x.size(1) <= 16384,
               "block_norm: the width must be 1..16384, got ", x.size(1));
   a.rows = x.size(0), a.D = x.size(1);
   a.x = x.data_ptr();
-  a.res = res.data_ptr();
+  a.res = res.has_value() ? res->data_ptr() : nullptr;
   bool seen = false;
   if (gate.has_value()) {
     if (gate->dim() == 1) {
@@ -212,7 +213,8 @@ unsigned grid_of(bool bwd, const torch::Tensor& x, const NormPlan& pl,
 
 // returns (s, h, stat): h is empty without pre_scale, stat without want_stat
 std::vector<torch::Tensor> block_norm_fwd(
-    torch::Tensor x, torch::Tensor res, c10::optional<torch::Tensor> gate,
+    torch::Tensor x, c10::optional<torch::Tensor> res,
+    c10::optional<torch::Tensor> gate,
     bool highway, double alpha, c10::optional<torch::Tensor> post_scale,
     c10::optional<torch::Tensor> post_bias,
     c10::optional<torch::Tensor> pre_scale,
@@ -237,7 +239,8 @@ std::vector<torch::Tensor> block_norm_fwd(
 // returns (dx, dres, dgate, dpost_scale, dpost_bias, dpre_scale, dpre_bias);
 // those that `want` (same order) does not ask for are empty
 std::vector<torch::Tensor> block_norm_bwd(
-    torch::Tensor x, torch::Tensor res, c10::optional<torch::Tensor> gate,
+    torch::Tensor x, c10::optional<torch::Tensor> res,
+    c10::optional<torch::Tensor> gate,
     bool highway, double alpha, c10::optional<torch::Tensor> post_scale,
     c10::optional<torch::Tensor> post_bias,
     c10::optional<torch::Tensor> pre_scale,
@@ -268,7 +271,7 @@ std::vector<torch::Tensor> block_norm_bwd(
   auto none = torch::empty({0}, x.options());
   std::vector<torch::Tensor> out(7, none);
   if (want[0]) out[0] = torch::empty_like(x), a.dx = out[0].data_ptr();
-  if (want[1]) out[1] = torch::empty_like(x), a.dres = out[1].data_ptr();
+  if (want[1] && a.res) out[1] = torch::empty_like(x), a.dres = out[1].data_ptr();
   const bool channel = is_channel(pl.gate);
   if (want[2] && is_token(pl.gate))
     out[2] = torch::empty_like(x), a.dgate = out[2].data_ptr();

@@ -18,13 +18,13 @@ Tensor gated_scan_bwd(Tensor x, Tensor gate, OptTensor state, OptTensor lens,
                       bool relu, Tensor dx, Tensor dgate, bool want_dstate);
 Tensor gated_step_fwd(Tensor x, Tensor gate, Tensor state, Tensor state_out,
                       bool relu);
-std::vector<Tensor> block_norm_fwd(Tensor x, Tensor res, OptTensor gate,
+std::vector<Tensor> block_norm_fwd(Tensor x, OptTensor res, OptTensor gate,
                                    bool highway, double alpha,
                                    OptTensor post_scale, OptTensor post_bias,
                                    OptTensor pre_scale, OptTensor pre_bias,
                                    bool rms, double eps, bool want_stat);
 std::vector<Tensor> block_norm_bwd(
-    Tensor x, Tensor res, OptTensor gate, bool highway, double alpha,
+    Tensor x, OptTensor res, OptTensor gate, bool highway, double alpha,
     OptTensor post_scale, OptTensor post_bias, OptTensor pre_scale,
     OptTensor pre_bias, bool rms, double eps, Tensor stat, OptTensor dsum,
     OptTensor dh, std::vector<bool> want);
@@ -171,17 +171,17 @@ OptTensor rows(const OptTensor& t, bool channel) {
   return !t.has_value() || channel ? t : OptTensor(rows(*t));
 }
 
-// x, res and a per-token gate: dense, of one shape
+// x, res (or none) and a per-token gate: dense, of one shape
 struct JoinFn : public torch::autograd::Function<JoinFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x,
-                               const Tensor& res, const OptTensor& gate,
+                               const OptTensor& res, const OptTensor& gate,
                                const OptTensor& w1, const OptTensor& b1,
                                const OptTensor& w2, const OptTensor& b2,
                                bool channel, bool highway, double alpha,
                                bool rms, double eps) {
-    auto out = block_norm_fwd(rows(x), rows(res), rows(gate, channel), highway,
-                              alpha, w1, b1, w2, b2, rms, eps, true);
-    ctx->save_for_backward({x, res, plain(gate), plain(w1), plain(b1),
+    auto out = block_norm_fwd(rows(x), rows(res, false), rows(gate, channel),
+                              highway, alpha, w1, b1, w2, b2, rms, eps, true);
+    ctx->save_for_backward({x, plain(res), plain(gate), plain(w1), plain(b1),
                             plain(w2), plain(b2), out[2]});
     ctx->saved_data["channel"] = channel;
     ctx->saved_data["highway"] = highway;
@@ -205,7 +205,7 @@ struct JoinFn : public torch::autograd::Function<JoinFn> {
                                             : OptTensor();
     };
     auto out = block_norm_bwd(
-        rows(s[0]), rows(s[1]), rows(opt(s[2]), channel),
+        rows(s[0]), rows(opt(s[1]), false), rows(opt(s[2]), channel),
         ctx->saved_data["highway"].toBool(),
         ctx->saved_data["alpha"].toDouble(), opt(s[3]), opt(s[4]), opt(s[5]),
         opt(s[6]), ctx->saved_data["rms"].toBool(),
@@ -262,7 +262,7 @@ std::tuple<Tensor, Tensor> gated_step(Tensor x, Tensor gate, OptTensor state_,
 }
 
 std::tuple<Tensor, OptTensor> block_norm(
-    Tensor x, Tensor res, OptTensor gate_, std::string gate_kind, double alpha,
+    Tensor x, OptTensor res_, OptTensor gate_, std::string gate_kind, double alpha,
     OptTensor post_scale, OptTensor post_bias, OptTensor pre_scale,
     OptTensor pre_bias, std::string norm, double eps) {
   REFUSE_UNLESS(x.dim() >= 1 && dtype_ok(x),
@@ -271,15 +271,19 @@ std::tuple<Tensor, OptTensor> block_norm(
   const int64_t D = x.size(-1);
   REFUSE_UNLESS(D > 0 && D <= 16384,
                 "block_norm: the width must be 1..16384, got ", D);
-  REFUSE_UNLESS(res.sizes() == x.sizes() &&
-                    res.scalar_type() == x.scalar_type() &&
-                    res.device() == x.device(),
-                "block_norm: res must have x's shape, dtype and device");
+  Tensor res = plain(res_);
+  if (res.defined())
+    REFUSE_UNLESS(res.sizes() == x.sizes() &&
+                      res.scalar_type() == x.scalar_type() &&
+                      res.device() == x.device(),
+                  "block_norm: res must have x's shape, dtype and device");
   REFUSE_UNLESS(norm == "layer" || norm == "rms",
                 "block_norm: norm must be layer or rms, got '", norm, "'");
   REFUSE_UNLESS(gate_kind == "scale" || gate_kind == "highway",
                 "block_norm: gate_kind must be scale or highway, got '",
                 gate_kind, "'");
+  REFUSE_UNLESS(res.defined() || gate_kind != "highway",
+                "block_norm: a highway needs res");
   Tensor gate = plain(gate_);
   bool channel_gate = false;
   if (gate.defined()) {
@@ -315,18 +319,18 @@ std::tuple<Tensor, OptTensor> block_norm(
   else if (gate.defined())
     gate = gate.contiguous();
   x = x.contiguous();
-  res = res.contiguous();
+  if (res.defined()) res = res.contiguous();
   const bool highway = gate_kind == "highway", rms = norm == "rms";
   bool grad = wants_grad(x) || wants_grad(res) || wants_grad(gate);
   for (auto& v : vec) grad = grad || wants_grad(v);
   if (grad && c10::GradMode::is_enabled()) {
-    auto out = JoinFn::apply(x, res, opt(gate), opt(vec[0]), opt(vec[1]),
+    auto out = JoinFn::apply(x, opt(res), opt(gate), opt(vec[0]), opt(vec[1]),
                              opt(vec[2]), opt(vec[3]), channel_gate, highway,
                              alpha, rms, eps);
     return {out[0], out.size() > 1 ? OptTensor(out[1]) : OptTensor()};
   }
   const at::NoGradGuard no_grad;
-  auto out = block_norm_fwd(rows(x), rows(res), rows(opt(gate), channel_gate),
+  auto out = block_norm_fwd(rows(x), rows(opt(res), false), rows(opt(gate), channel_gate),
                             highway, alpha, opt(vec[0]), opt(vec[1]),
                             opt(vec[2]), opt(vec[3]), rms, eps, false);
   return {out[0].view(x.sizes()),

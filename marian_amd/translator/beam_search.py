@@ -97,8 +97,9 @@ class BeamSearch:
             if isinstance(model, TransformerModel) \
                     and model.compute_dtype == torch.bfloat16 \
                     and model.decoder and model.decoder[0].autoreg \
-                    == "self-attention" \
-                    and model.dim // model.decoder[0].self_attn.heads == 64:
+                    in ("self-attention", "rnn") \
+                    and model.decoder[0].context_attn is not None \
+                    and model.decoder[0].context_attn.dh == 64:
                 try:
                     from .graph_decode import GraphedDecodeStep
                     sup = -1 if self.allow_unk else self.unk_id

@@ -12,7 +12,8 @@ gathers A->B on even steps and B->A on odd steps, so every tensor address
 the graph baked stays valid).
 
 Requirements (checked; eager fallback otherwise): single scorer,
-TransformerModel, bf16 on cuda, Dh=64 (the fused attention kernel),
+TransformerModel (attention or recurrent decoder), bf16 on cuda, Dh=64 (the
+fused attention kernel),
 post-norm or prenorm without dropout, no alignment collection / sampling /
 shortlist.
 
@@ -27,7 +28,7 @@ import torch
 
 from .. import ops
 from ..models.transformer import TransformerModel, NEG_INF
-from ..models.layers import sinusoidal_position_embeddings
+from ..models.layers import join_blocks, sinusoidal_position_embeddings
 
 
 class GraphedDecodeStep:
@@ -47,8 +48,10 @@ class GraphedDecodeStep:
         self.device = dev
         self.dt = dt
         L = len(model.decoder)
-        H = model.decoder[0].self_attn.heads
-        dh = model.decoder[0].self_attn.dh
+        # recurrent decoders keep a state per layer in place of a KV cache
+        self.rnn = model.decoder[0].autoreg == "rnn"
+        H = model.decoder[0].context_attn.heads
+        dh = model.decoder[0].context_attn.dh
         d = model.dim
         self.L, self.H, self.dh, self.d = L, H, dh, d
 
@@ -64,9 +67,11 @@ class GraphedDecodeStep:
         self.step_t = torch.zeros(1, dtype=torch.long, device=dev)
         self.kv_lens = torch.zeros(n_rows, dtype=torch.int32, device=dev)
         self.scores = torch.zeros(n_rows, dtype=torch.float32, device=dev)
-        # ping-pong KV buffers [2(k/v), L, N, H, Tmax, dh]
-        self.kv = [torch.zeros(2, L, n_rows, H, max_len, dh, device=dev,
-                               dtype=dt) for _ in range(2)]
+        # ping-pong buffers: KV [2(k/v), L, N, H, Tmax, dh] or, for recurrent
+        # decoders, float32 states [1, L, N, d]; rows in dim 2 of both
+        self.kv = [torch.zeros(1, L, n_rows, d, device=dev) if self.rnn
+                   else torch.zeros(2, L, n_rows, H, max_len, dh, device=dev,
+                                    dtype=dt) for _ in range(2)]
         # precomputed positional table
         self.pos_table = sinusoidal_position_embeddings(
             max_len + 1, d, device=dev, dtype=dt)
@@ -138,24 +143,25 @@ class GraphedDecodeStep:
         for i, layer in enumerate(m.decoder):
             h = layer.pre_self(x)
             a = layer.self_attn
-            qkv = ops.linear(h, a.W_qkv, a.b_qkv)
-            qh, kh, vh = qkv.split(d, dim=-1)
-            q = a._split(qh)           # [N, H, 1, dh]
-            # write this step's K/V at position `step` (dim 2 of [N,H,T,dh])
-            kv_dst[0, i].index_copy_(2, self.step_t, a._split(kh))
-            kv_dst[1, i].index_copy_(2, self.step_t, a._split(vh))
-            att = ops.attention(q, kv_dst[0, i], kv_dst[1, i],
-                                lens=self.kv_lens)
-            h = a.Wo(a._join(att))
-            x = layer.post_self(h, residual=x)
-            h = layer.pre_ctx(x)
+            if self.rnn:
+                h = a.step(h[:, 0], kv_dst[0, i], inplace=True)[0][:, None]
+            else:
+                qkv = ops.linear(h, a.W_qkv, a.b_qkv)
+                qh, kh, vh = qkv.split(d, dim=-1)
+                q = a._split(qh)       # [N, H, 1, dh]
+                # this step's K/V at position `step` (dim 2 of [N,H,T,dh])
+                kv_dst[0, i].index_copy_(2, self.step_t, a._split(kh))
+                kv_dst[1, i].index_copy_(2, self.step_t, a._split(vh))
+                att = ops.attention(q, kv_dst[0, i], kv_dst[1, i],
+                                    lens=self.kv_lens)
+                h = a.Wo(a._join(att))
+            x, h = join_blocks(layer.post_self, layer.pre_ctx, h, x)
             ca = layer.context_attn
             q2 = ca._split(ops.linear(h, ca.w_slice(0), ca.b_slice(0)))
             att2 = ops.attention(q2, self.cross_k[i], self.cross_v[i],
                                  mask=self.src_lmask, lens=self.src_lens)
             h = ca.Wo(ca._join(att2))
-            x = layer.post_ctx(h, residual=x)
-            h = layer.pre_ffn(x)
+            x, h = join_blocks(layer.post_ctx, layer.pre_ffn, h, x)
             h = layer.ffn(h)
             x = layer.post_ffn(h, residual=x)
         if m.post_top_dec is not None:
@@ -216,6 +222,9 @@ class GraphedDecodeStep:
         """Prepare for a fresh decode: the first replay runs step 0 with a
         zero embedding (emb_scale=0) and only beam 0 live."""
         self.step_t.zero_()
+        if self.rnn:            # KV rows are hidden by kv_lens instead
+            for t in self.kv:
+                t.zero_()
         self.kv_lens.fill_(1)
         self.emb_scale.fill_(0.0)
         self.prev_tokens.zero_()

@@ -5,6 +5,7 @@
 The resulting marian_amd/ops/_hip_ext*.so is git-ignored but travels with
 gpurun snapshots to the GPU box.
 """
+import hashlib
 import os
 import sys
 
@@ -43,17 +44,27 @@ ltgemm = os.path.join(HIP_DIR, "ltgemm.cpp")
 if os.path.exists(ltgemm):
     sources.append(ltgemm)
 
+# The build tracks no headers for HIP sources: their contents go into the
+# command line, so that a change of one builds every object again. (A kernel
+# object that is older than its header may not fit the host code beside it.)
+headers = [os.path.join(HIP_DIR, name)
+           for name in ("common.h", "vec.h", "block_norm.h")]
+digest = hashlib.sha256()
+for path in headers:
+    with open(path, "rb") as f:
+        digest.update(f.read())
+
 ext = CUDAExtension(
     name="marian_amd.ops._hip_ext",
     sources=sources,
-    depends=[os.path.join(HIP_DIR, name)
-             for name in ("common.h", "vec.h", "block_norm.h")],
+    depends=headers,
     libraries=["hipblaslt"],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],
         # no packed fp32 instructions: some of their forms are not reliable
         "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950", "-Xclang",
-                 "-target-feature", "-Xclang", "-packed-fp32-ops"],
+                 "-target-feature", "-Xclang", "-packed-fp32-ops",
+                 "-DMAMD_HEADERS=" + digest.hexdigest()[:16]],
     },
 )
 

@@ -77,7 +77,8 @@ def oracle(t, norm, gate_kind, alpha, eps=1e-9):
         o = g - xh * (g * xh).mean()
         return (o - g.mean() if norm == "layer" else o) * r
 
-    x, res = d["x"], d["res"]
+    x = d["x"]
+    res = d["res"] or Num(torch.zeros_like(x.v))
     u, xh, xr = normed(x, "post") if d["post_scale"] is not None \
         else (x, None, None)
     one = Num(torch.ones(1, dtype=torch.float64))
@@ -109,12 +110,13 @@ def oracle(t, norm, gate_kind, alpha, eps=1e-9):
     return out
 
 
+# make(no_res=True): the residual's term is left out
 LEAVES = ("x", "res", "gate", "post_scale", "post_bias", "pre_scale",
           "pre_bias")
 
 
 def make(R, D, dtype, dev, norm="layer", gate=None, per_token=False, post=True,
-         pre=True, bias=True, pdt=None, seed=0, shift=0.5):
+         pre=True, bias=True, pdt=None, seed=0, shift=0.5, no_res=False):
     gen = torch.Generator().manual_seed(seed)
     rnd = lambda *s: torch.randn(*s, generator=gen)
     pdt = pdt or dtype
@@ -122,6 +124,8 @@ def make(R, D, dtype, dev, norm="layer", gate=None, per_token=False, post=True,
          "res": (rnd(R, D) * 3 - 0.5).to(dtype), "gate": None,
          "dsum": rnd(R, D).to(dtype),
          "dh": rnd(R, D).to(dtype) if pre else None}
+    if no_res:
+        t["res"] = None
     if gate:
         t["gate"] = (rnd(R, D) if per_token else rnd(D)).add(0.3).to(
             dtype if per_token else pdt)
@@ -178,6 +182,7 @@ CPU_CASES = [
     dict(R=4, D=16, dtype=torch.bfloat16, gate="highway", per_token=True),
     dict(R=4, D=16, dtype=torch.float32, gate="highway", post=False),
     dict(R=4, D=16, dtype=torch.float32, gate="scale", pre=False, alpha=0.7),
+    dict(R=4, D=9, dtype=torch.float32, norm="rms", pre=False, no_res=True),
 ]
 
 
@@ -219,6 +224,7 @@ def test_refusals(dev):
     refused(x, x, gate=zeros(3, 4))
     refused(x, x, gate=zeros(2, 1, 4))
     refused(x, x, gate=zeros(2, 3, 4).bfloat16())
+    refused(x, None, gate=x, gate_kind="highway")
     refused(x, x, post_bias=w)
     refused(x, x, pre_scale=w[:3])
     refused(x, x, pre_scale=w.double())
@@ -261,6 +267,10 @@ GPU_CASES = [
          gate="highway", alpha=0.5),
     dict(R=9, D=1000, dtype=torch.float32, pre=False, post=False,
          gate="scale", per_token=True),
+    dict(R=9, D=96, dtype=torch.float32, norm="rms", pre=False, no_res=True),
+    dict(R=9, D=700, dtype=torch.bfloat16, gate="scale", no_res=True),
+    dict(R=9, D=50, dtype=torch.float16, gate="scale", per_token=True,
+         post=False, pre=False, no_res=True),
     # a mean far from 0 beside the deviation
     dict(R=12, D=700, dtype=torch.float32, shift=300.0),
 ]
