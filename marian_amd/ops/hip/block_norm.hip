@@ -4,6 +4,7 @@
 #include <ATen/hip/HIPContext.h>
 
 #include "block_norm.h"
+#include "fresh.h"
 
 using namespace mamd;
 
@@ -211,7 +212,8 @@ unsigned grid_of(bool bwd, const torch::Tensor& x, const NormPlan& pl,
 
 }  // namespace
 
-// returns (s, h, stat): h is empty without pre_scale, stat without want_stat
+// returns (s, h, stat): h is undefined without pre_scale, stat without
+// want_stat
 std::vector<torch::Tensor> block_norm_fwd(
     torch::Tensor x, c10::optional<torch::Tensor> res,
     c10::optional<torch::Tensor> gate,
@@ -224,20 +226,21 @@ std::vector<torch::Tensor> block_norm_fwd(
                       pre_scale, pre_bias, rms, eps, false);
   NormArgs& a = pl.a;
   const c10::DeviceGuard guard(x.device());
-  auto s = torch::empty_like(x);
-  auto h = a.pre_scale ? torch::empty_like(x) : torch::empty({0}, x.options());
-  auto stat = torch::empty({want_stat ? 4 : 0, (long)a.rows},
-                           x.options().dtype(torch::kFloat32));
+  auto s = fresh_like(x);
+  torch::Tensor h, stat;
+  if (a.pre_scale) h = fresh_like(x), a.h = h.data_ptr();
+  if (want_stat) {
+    stat = fresh({4, a.rows}, torch::kFloat32, x);
+    a.stat = stat.data_ptr<float>();
+  }
   if (a.rows == 0) return {s, h, stat};
   a.s = s.data_ptr();
-  a.h = h.data_ptr();
-  a.stat = want_stat ? stat.data_ptr<float>() : nullptr;
   dispatch(false, x, pl, grid_of(false, x, pl, 1));
   return {s, h, stat};
 }
 
 // returns (dx, dres, dgate, dpost_scale, dpost_bias, dpre_scale, dpre_bias);
-// those that `want` (same order) does not ask for are empty
+// those that `want` (same order) does not ask for are undefined
 std::vector<torch::Tensor> block_norm_bwd(
     torch::Tensor x, c10::optional<torch::Tensor> res,
     c10::optional<torch::Tensor> gate,
@@ -268,18 +271,17 @@ std::vector<torch::Tensor> block_norm_bwd(
     check_like(dhc, x, "dh");
     a.dh = dhc.data_ptr();
   }
-  auto none = torch::empty({0}, x.options());
-  std::vector<torch::Tensor> out(7, none);
-  if (want[0]) out[0] = torch::empty_like(x), a.dx = out[0].data_ptr();
-  if (want[1] && a.res) out[1] = torch::empty_like(x), a.dres = out[1].data_ptr();
+  std::vector<torch::Tensor> out(7);
+  if (want[0]) out[0] = fresh_like(x), a.dx = out[0].data_ptr();
+  if (want[1] && a.res) out[1] = fresh_like(x), a.dres = out[1].data_ptr();
   const bool channel = is_channel(pl.gate);
   if (want[2] && is_token(pl.gate))
-    out[2] = torch::empty_like(x), a.dgate = out[2].data_ptr();
+    out[2] = fresh_like(x), a.dgate = out[2].data_ptr();
   SumArgs sm{};
-  auto popt = x.options().dtype(a.param32 ? torch::kFloat32 : x.scalar_type());
+  const auto pdt = a.param32 ? torch::kFloat32 : x.scalar_type();
   auto vec = [&](int at, bool there) {
     if (!want[at] || !there) return false;
-    out[at] = torch::empty({a.D}, popt);
+    out[at] = fresh({a.D}, pdt, x);
     sm.out[at - 2] = out[at].data_ptr();
     return true;
   };
@@ -291,7 +293,8 @@ std::vector<torch::Tensor> block_norm_bwd(
   for (int p = 0; p < kNumSums; ++p)
     sm.slot[p] = a.slot[p] = use[p] ? a.n_part++ : -1;
   if (a.rows == 0) {
-    for (auto& t : out) t.zero_();
+    for (auto& t : out)
+      if (t.defined()) t.zero_();
     return out;
   }
   // 4 turns at least for each block: one turn's partial sums are as many
@@ -299,8 +302,7 @@ std::vector<torch::Tensor> block_norm_bwd(
   const unsigned grid = grid_of(true, x, pl, a.n_part ? 4 : 1);
   torch::Tensor part;
   if (a.n_part) {
-    part = torch::empty({(long)grid, a.n_part, a.D},
-                        x.options().dtype(torch::kFloat32));
+    part = fresh({(long)grid, a.n_part, a.D}, torch::kFloat32, x);
     a.part = part.data_ptr<float>();
   }
   dispatch(true, x, pl, grid);

@@ -5,6 +5,8 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include "fresh.h"
+
 using torch::Tensor;
 using OptTensor = c10::optional<Tensor>;
 using torch::autograd::AutogradContext;
@@ -130,16 +132,15 @@ struct ScanFn : public torch::autograd::Function<ScanFn> {
     // absent inputs have no edge
     const bool want_state =
         s[2].defined() && ctx->needs_input_grad(fused ? 1 : 2);
-    Tensor dx = torch::empty(s[0].sizes(), s[0].options());
-    Tensor dg = fused ? Tensor() : torch::empty(s[0].sizes(), s[0].options());
+    Tensor dx = mamd::fresh_like(s[0]);
+    Tensor dg = fused ? Tensor() : mamd::fresh_like(s[0]);
     auto ds = gated_scan_bwd(
         fused ? half(s[0], 0) : s[0], fused ? half(s[0], 1) : s[1], opt(s[2]),
         opt(s[3]), s[4], opt(g[0]),
         g[1].defined() ? OptTensor(g[1].contiguous()) : OptTensor(),
         ctx->saved_data["reverse"].toBool(), ctx->saved_data["relu"].toBool(),
         fused ? half(dx, 0) : dx, fused ? half(dx, 1) : dg, want_state);
-    return once({dx, dg, want_state ? ds : Tensor(), Tensor(), Tensor(),
-                 Tensor()});
+    return once({dx, dg, ds, Tensor(), Tensor(), Tensor()});
   }
 };
 
@@ -167,6 +168,10 @@ std::tuple<Tensor, Tensor> scan(Tensor x, Tensor gate, Tensor state,
 Tensor rows(const Tensor& t) {
   return t.dim() == 2 ? t : t.view({t.numel() / t.size(-1), t.size(-1)});
 }
+// the other way round
+Tensor like(const Tensor& rows, const Tensor& t) {
+  return t.dim() == rows.dim() ? rows : rows.view(t.sizes());
+}
 OptTensor rows(const OptTensor& t, bool channel) {
   return !t.has_value() || channel ? t : OptTensor(rows(*t));
 }
@@ -189,8 +194,8 @@ struct JoinFn : public torch::autograd::Function<JoinFn> {
     ctx->saved_data["rms"] = rms;
     ctx->saved_data["eps"] = eps;
     ctx->set_materialize_grads(false);
-    if (!w2.has_value()) return {out[0].view(x.sizes())};
-    return {out[0].view(x.sizes()), out[1].view(x.sizes())};
+    if (!w2.has_value()) return {like(out[0], x)};
+    return {like(out[0], x), like(out[1], x)};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list g) {
@@ -210,8 +215,8 @@ struct JoinFn : public torch::autograd::Function<JoinFn> {
         ctx->saved_data["alpha"].toDouble(), opt(s[3]), opt(s[4]), opt(s[5]),
         opt(s[6]), ctx->saved_data["rms"].toBool(),
         ctx->saved_data["eps"].toDouble(), s[7], grad(0), grad(1), want);
-    for (size_t i = 0; i < 7; ++i)
-      out[i] = want[i] ? out[i].view(s[i].sizes()) : Tensor();
+    for (size_t i = 0; i < 3; ++i)
+      if (out[i].defined()) out[i] = like(out[i], s[i]);
     out.resize(12);
     return once(std::move(out));
   }
@@ -256,7 +261,7 @@ std::tuple<Tensor, Tensor> gated_step(Tensor x, Tensor gate, OptTensor state_,
     return {std::get<0>(out).squeeze(1), std::get<1>(out)};
   }
   state = state.contiguous();
-  Tensor out = inplace ? state : torch::empty_like(state);
+  Tensor out = inplace ? state : mamd::fresh_like(state);
   return {gated_step_fwd(dense_rows(x), dense_rows(gate), state, out, relu),
           out};
 }
@@ -333,6 +338,6 @@ std::tuple<Tensor, OptTensor> block_norm(
   auto out = block_norm_fwd(rows(x), rows(opt(res), false), rows(opt(gate), channel_gate),
                             highway, alpha, opt(vec[0]), opt(vec[1]),
                             opt(vec[2]), opt(vec[3]), rms, eps, false);
-  return {out[0].view(x.sizes()),
-          vec[2].defined() ? OptTensor(out[1].view(x.sizes())) : OptTensor()};
+  return {like(out[0], x),
+          vec[2].defined() ? OptTensor(like(out[1], x)) : OptTensor()};
 }

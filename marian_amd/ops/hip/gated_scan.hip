@@ -21,6 +21,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "fresh.h"
 #include "vec.h"
 
 using namespace mamd;
@@ -743,8 +744,7 @@ void run(bool bwd, const torch::Tensor& x, ScanArgs& a) {
   auto stream = at::cuda::getCurrentHIPStream();
   torch::Tensor agg;
   if (a.nc > 1) {
-    agg = torch::empty({2, a.B, a.nc, a.D},
-                       x.options().dtype(torch::kFloat32));
+    agg = fresh({2, a.B, a.nc, a.D}, torch::kFloat32, x);
     a.agg = agg.data_ptr<float>();
     launch<true>(bwd, x, a, stream);
   }
@@ -753,7 +753,7 @@ void run(bool bwd, const torch::Tensor& x, ScanArgs& a) {
 
 }  // namespace
 
-// returns (y, last, bnd); bnd is empty unless want_bnd and T spans tiles
+// returns (y, last, bnd); bnd is undefined unless want_bnd and T spans tiles
 std::vector<torch::Tensor> gated_scan_fwd(torch::Tensor x, torch::Tensor gate,
                                           c10::optional<torch::Tensor> state,
                                           c10::optional<torch::Tensor> lens,
@@ -761,12 +761,11 @@ std::vector<torch::Tensor> gated_scan_fwd(torch::Tensor x, torch::Tensor gate,
                                           bool want_bnd) {
   ScanArgs a = base_args(x, gate, state, lens, reverse, relu);
   const c10::DeviceGuard guard(x.device());
-  auto f32 = x.options().dtype(torch::kFloat32);
-  auto y = torch::empty({a.B, a.T, a.D}, x.options());
-  auto last = torch::empty({a.B, a.D}, f32);
-  auto bnd = torch::empty({0}, f32);
+  auto y = fresh_like(x);
+  auto last = fresh({a.B, a.D}, torch::kFloat32, x);
+  torch::Tensor bnd;
   if (want_bnd && a.nt > 1) {
-    bnd = torch::empty({a.B, a.nt, a.D}, f32);
+    bnd = fresh({a.B, a.nt, a.D}, torch::kFloat32, x);
     a.bnd = bnd.data_ptr<float>();
   }
   a.y = y.data_ptr();
@@ -776,7 +775,7 @@ std::vector<torch::Tensor> gated_scan_fwd(torch::Tensor x, torch::Tensor gate,
   return {y, last, bnd};
 }
 
-// writes dx and dgate (any batch and time strides); returns dstate, empty
+// writes dx and dgate (any batch and time strides); returns dstate, undefined
 // unless want_dstate
 torch::Tensor gated_scan_bwd(torch::Tensor x, torch::Tensor gate,
                              c10::optional<torch::Tensor> state,
@@ -793,7 +792,7 @@ torch::Tensor gated_scan_bwd(torch::Tensor x, torch::Tensor gate,
                   dx.scalar_type() == x.scalar_type(),
               "gated_scan_bwd: dx must be like x");
   if (a.nt > 1) {
-    TORCH_CHECK(bnd.device() == x.device() &&
+    TORCH_CHECK(bnd.defined() && bnd.device() == x.device() &&
                     bnd.scalar_type() == torch::kFloat32 &&
                     bnd.is_contiguous() && bnd.dim() == 3 &&
                     bnd.size(0) == a.B && bnd.size(1) == a.nt &&
@@ -814,10 +813,11 @@ torch::Tensor gated_scan_bwd(torch::Tensor x, torch::Tensor gate,
   a.dg = dgate.data_ptr();
   a.dxb = dx.stride(0), a.dxt = time_stride(dx);
   a.dgb = dgate.stride(0), a.dgt = time_stride(dgate);
-  auto f32 = x.options().dtype(torch::kFloat32);
-  auto dstate = want_dstate ? torch::empty({a.B, a.D}, f32)
-                            : torch::empty({0}, f32);
-  if (want_dstate) a.dstate = dstate.data_ptr<float>();
+  torch::Tensor dstate;
+  if (want_dstate) {
+    dstate = fresh({a.B, a.D}, torch::kFloat32, x);
+    a.dstate = dstate.data_ptr<float>();
+  }
   if (a.B == 0) return dstate;
   run(true, x, a);
   return dstate;
@@ -834,7 +834,7 @@ torch::Tensor gated_step_fwd(torch::Tensor x, torch::Tensor gate,
   const c10::DeviceGuard guard(x.device());
   const long N = x.size(0), D = x.size(1);
   TORCH_CHECK(D < (1L << 30), "gated_step: the width must stay below 2^30");
-  auto y = torch::empty({N, D}, x.options());
+  auto y = fresh_like(x);
   if (N == 0) return y;
   auto stream = at::cuda::getCurrentHIPStream();
   const int vpr = (int)((D + 3) / 4);

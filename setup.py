@@ -48,7 +48,7 @@ if os.path.exists(ltgemm):
 # command line, so that a change of one builds every object again. (A kernel
 # object that is older than its header may not fit the host code beside it.)
 headers = [os.path.join(HIP_DIR, name)
-           for name in ("common.h", "vec.h", "block_norm.h")]
+           for name in ("common.h", "vec.h", "fresh.h", "block_norm.h")]
 digest = hashlib.sha256()
 for path in headers:
     with open(path, "rb") as f:
