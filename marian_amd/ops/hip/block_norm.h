@@ -256,8 +256,9 @@ __device__ __forceinline__ void coefs(float alpha, float gt, float& ca,
 // mean and 1/deviation of a row
 template <int VEC, int NC, int PLACE>
 __device__ __forceinline__ void stats(const float* v,
-                                      const Columns<VEC, NC>& c, int D,
-                                      int rms, float eps, RowSum<PLACE>& sum,
+                                      const Columns<VEC, NC>& c,
+                                      float inv_d, int rms, float eps,
+                                      RowSum<PLACE>& sum,
                                       float& mean, float& rstd) {
   mean = 0.f;
   if (!rms) {
@@ -265,7 +266,7 @@ __device__ __forceinline__ void stats(const float* v,
 #pragma unroll
     for (int e = 0; e < VEC * NC; ++e) p += c.own(e) ? v[e] : 0.f;
     sum(p);
-    mean = p / D;
+    mean = p * inv_d;
   }
   float q = 0.f;
 #pragma unroll
@@ -274,7 +275,7 @@ __device__ __forceinline__ void stats(const float* v,
     q += d * d;
   }
   sum(q);
-  rstd = 1.f / sqrtf(q / D + eps);
+  rstd = rsqrtf(q * inv_d + eps);
 }
 
 // the rows of a lane group, and the next of them
@@ -315,6 +316,7 @@ __global__ __launch_bounds__(MAXT) void join_fwd_kernel(NormArgs a) {
   using Raw = RawRow<T, VEC, NC>;
   __shared__ float buf[2][32];
   RowSum<PLACE> sum(buf, a.tpr);
+  const float inv_d = 1.f / (float)a.D;
   const Rows<PLACE> it(a);
   const Columns<VEC, NC> col(it.lane, a.tpr, a.D);
   const Param<T, VEC, NC, KEEP> w1(POST ? a.post_scale : nullptr, a.param32, 1.f,
@@ -340,7 +342,7 @@ __global__ __launch_bounds__(MAXT) void join_fwd_kernel(NormArgs a) {
     const long row = it.row + r0 * it.stride;
     if (PLACE != kPartWave && row >= a.rows) break;
     if (!KEEP) fetch(row);
-    const bool on = row < a.rows;
+    const bool on = PLACE != kPartWave || row < a.rows;
     const long base = row * a.D;
     float x[EPT], s[EPT], gt[EPT], w[EPT], bb[EPT];
 #pragma unroll
@@ -353,7 +355,7 @@ __global__ __launch_bounds__(MAXT) void join_fwd_kernel(NormArgs a) {
     if constexpr (is_channel(GATE)) gp.get(col, gt);
     float m1 = 0.f, r1 = 1.f, m2 = 0.f, r2 = 1.f;
     if constexpr (POST) {
-      stats<VEC, NC, PLACE>(x, col, a.D, a.rms, a.eps, sum, m1, r1);
+      stats<VEC, NC, PLACE>(x, col, inv_d, a.rms, a.eps, sum, m1, r1);
       w1.get(col, w);
       b1.get(col, bb);
 #pragma unroll
@@ -372,7 +374,7 @@ __global__ __launch_bounds__(MAXT) void join_fwd_kernel(NormArgs a) {
           store_vec<T, VEC>((T*)a.s + base + col.at[i], s + i * VEC);
     }
     if constexpr (PRE) {
-      stats<VEC, NC, PLACE>(s, col, a.D, a.rms, a.eps, sum, m2, r2);
+      stats<VEC, NC, PLACE>(s, col, inv_d, a.rms, a.eps, sum, m2, r2);
       w2.get(col, w);
       b2.get(col, bb);
 #pragma unroll
@@ -400,11 +402,14 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
   // blocks of 1024 have 128 registers a lane: parameters are read again for
   // each row and nothing is fetched ahead
   constexpr bool KEEP = MAXT <= 512;
+  // rows of 16 elements a lane leave no registers for the next row's
+  constexpr bool AHEAD = KEEP && !(PLACE == kBlock && EPT == 16);
   using Raw = RawRow<T, VEC, NC>;
   __shared__ float buf[2][32];
   // the lane groups' sums of one parameter
   __shared__ float fold[PLACE == kBlock ? 1 : EPT * 256];
   RowSum<PLACE> sum(buf, a.tpr);
+  const float inv_d = 1.f / (float)a.D;
   const Rows<PLACE> it(a);
   const Columns<VEC, NC> col(it.lane, a.tpr, a.D);
   const Param<T, VEC, NC, KEEP> w1(POST ? a.post_scale : nullptr, a.param32, 1.f,
@@ -439,12 +444,12 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) st[i] = a.stat[i * a.rows + row];
   };
-  if (KEEP) fetch(it.row);
+  if (AHEAD) fetch(it.row);
   for (long r0 = 0, n = (a.rows + it.stride - 1) / it.stride; r0 < n; ++r0) {
     const long row = it.row + r0 * it.stride;
     if (PLACE != kPartWave && row >= a.rows) break;
-    if (!KEEP) fetch(row);
-    const bool on = row < a.rows;
+    if (!AHEAD) fetch(row);
+    const bool on = PLACE != kPartWave || row < a.rows;
     const long base = row * a.D;
     // this row, 16-bit values kept as they are until they are used
     const Raw rc = rr, dc = dr, hc = hr, gc = gr;
@@ -453,7 +458,7 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
 #pragma unroll
     for (int e = 0; e < EPT; ++e)  // the normalised row
       x[e] = POST ? (xr[e] - m1) * r1 : NEED ? xr[e] : 0.f;
-    if (KEEP && r0 + 1 < n) fetch(row + it.stride);
+    if (AHEAD && r0 + 1 < n) fetch(row + it.stride);
     auto gates = [&]() __attribute__((always_inline)) {
       if constexpr (is_channel(GATE)) gp.get(col, gt);
 #pragma unroll
@@ -482,8 +487,8 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
         q += col.own(e) ? gh[e] * sh[e] : 0.f;
       }
       sum(p, q);
-      p = a.rms ? 0.f : p / a.D;
-      q /= a.D;
+      p = a.rms ? 0.f : p * inv_d;
+      q *= inv_d;
 #pragma unroll
       for (int e = 0; e < EPT; ++e)
         ds[e] = (on ? dc[e] : 0.f) + r2 * (gh[e] - p - sh[e] * q);
@@ -529,8 +534,8 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
     if constexpr (is_token(GATE)) put(a.dgate, gt);
     if constexpr (POST) {
       sum(p, q);
-      p = a.rms ? 0.f : p / a.D;
-      q /= a.D;
+      p = a.rms ? 0.f : p * inv_d;
+      q *= inv_d;
 #pragma unroll
       for (int e = 0; e < EPT; ++e) ds[e] = r1 * (ds[e] - p - x[e] * q);
     }
