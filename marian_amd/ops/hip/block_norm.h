@@ -80,8 +80,12 @@ struct NormArgs {
   int slot[kNumSums];        // a sum's row in part, or -1
 };
 
-// How a row's lanes are placed: some lanes of a wave, one wave, or a block.
-enum { kPartWave = 0, kWave = 1, kBlock = 2 };
+// How a row's lanes are placed: some lanes of a wave, one wave, two of a
+// block's four waves, or a block.
+enum { kPartWave = 0, kWave = 1, kPair = 2, kBlock = 3 };
+// lane groups that may be without a row while others of their wave or block
+// still have one
+constexpr bool may_idle(int place) { return place == kPartWave || place == kPair; }
 
 // sum over a wave in a fixed order, in all lanes: 4 steps inside rows of 16
 // lanes and 2 between them, all of them modifiers of an add
@@ -117,13 +121,19 @@ struct RowSum {
       p = dpp_sum(p);
       q = dpp_sum(q);
     }
-    if constexpr (PLACE == kBlock) {
-      const int nw = tpr / WAVE, wid = threadIdx.x / WAVE;
+    if constexpr (PLACE == kPair || PLACE == kBlock) {
+      const int wid = threadIdx.x / WAVE;
       if (threadIdx.x % WAVE == 0)
         buf[flip][wid] = p, buf[flip][16 + wid] = q;
       __syncthreads();
-      p = q = 0.f;
-      for (int i = 0; i < nw; ++i) p += buf[flip][i], q += buf[flip][16 + i];
+      if constexpr (PLACE == kPair) {
+        const float* w = &buf[flip][wid & ~1];
+        p = w[0] + w[1], q = w[16] + w[17];
+      } else {
+        const int nw = tpr / WAVE;
+        p = q = 0.f;
+        for (int i = 0; i < nw; ++i) p += buf[flip][i], q += buf[flip][16 + i];
+      }
       flip ^= 1;
     }
   }
@@ -278,34 +288,32 @@ __device__ __forceinline__ void stats(const float* v,
   rstd = rsqrtf(q * inv_d + eps);
 }
 
-// the rows of a lane group, and the next of them
+// the rows of a lane group: row, row + stride, ...; row0 is its block's first
 template <int PLACE>
 struct Rows {
-  long row, stride;
+  long row, row0, stride;
   int lane;
   __device__ __forceinline__ Rows(const NormArgs& a) {
-    if constexpr (PLACE == kPartWave) {
+    if constexpr (PLACE == kBlock) {
+      lane = threadIdx.x;
+      row = row0 = blockIdx.x;
+      stride = gridDim.x;
+    } else {
       const int rpb = blockDim.x / a.tpr;
       lane = threadIdx.x & (a.tpr - 1);
-      row = (long)blockIdx.x * rpb + threadIdx.x / a.tpr;
+      int group = threadIdx.x / a.tpr;
+      if constexpr (PLACE != kPartWave)
+        group = __builtin_amdgcn_readfirstlane(group);
+      row0 = (long)blockIdx.x * rpb;
+      row = row0 + group;
       stride = (long)gridDim.x * rpb;
-    } else if constexpr (PLACE == kWave) {
-      const int rpb = blockDim.x / WAVE;
-      lane = threadIdx.x & (WAVE - 1);
-      row = (long)blockIdx.x * rpb +
-            __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-      stride = (long)gridDim.x * rpb;
-    } else {
-      lane = threadIdx.x;
-      row = blockIdx.x;
-      stride = gridDim.x;
     }
   }
 };
 
-// Lanes without a row (the end of the last block, part-wave placement only
-// mixes them with others) work on the last row and store nothing; sums never
-// leave a lane group, so they cost the others nothing but time.
+// Lane groups without a row (at the end of the last block) work on the last
+// row, in the backward pass on zeros, and store nothing; a row's sums never
+// leave its lane group.
 template <typename T, int VEC, int EPT, int PLACE, bool POST, bool PRE,
           int GATE, int MAXT>
 __global__ __launch_bounds__(MAXT) void join_fwd_kernel(NormArgs a) {
@@ -340,9 +348,12 @@ __global__ __launch_bounds__(MAXT) void join_fwd_kernel(NormArgs a) {
   // the same number of turns for all lanes of a wave
   for (long r0 = 0, n = (a.rows + it.stride - 1) / it.stride; r0 < n; ++r0) {
     const long row = it.row + r0 * it.stride;
-    if (PLACE != kPartWave && row >= a.rows) break;
+    // waves that meet at barriers leave together
+    if ((PLACE == kPair ? it.row0 + r0 * it.stride : row) >= a.rows &&
+        PLACE != kPartWave)
+      break;
     if (!KEEP) fetch(row);
-    const bool on = PLACE != kPartWave || row < a.rows;
+    const bool on = !may_idle(PLACE) || row < a.rows;
     const long base = row * a.D;
     float x[EPT], s[EPT], gt[EPT], w[EPT], bb[EPT];
 #pragma unroll
@@ -432,6 +443,12 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
   float st[4];
   rr.zero();
   auto fetch = [&](long row) __attribute__((always_inline)) {
+    if (may_idle(PLACE) && row >= a.rows) {  // zeros add nothing to the sums
+      xr.zero(), rr.zero(), dr.zero(), hr.zero(), gr.zero();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) st[i] = 0.f;
+      return;
+    }
     row = min(row, a.rows - 1);
     const long base = row * a.D;
     if constexpr (POST || NEED) xr.load((const T*)a.x + base, col);
@@ -447,9 +464,12 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
   if (AHEAD) fetch(it.row);
   for (long r0 = 0, n = (a.rows + it.stride - 1) / it.stride; r0 < n; ++r0) {
     const long row = it.row + r0 * it.stride;
-    if (PLACE != kPartWave && row >= a.rows) break;
+    // waves that meet at barriers leave together
+    if ((PLACE == kPair ? it.row0 + r0 * it.stride : row) >= a.rows &&
+        PLACE != kPartWave)
+      break;
     if (!AHEAD) fetch(row);
-    const bool on = PLACE != kPartWave || row < a.rows;
+    const bool on = !may_idle(PLACE) || row < a.rows;
     const long base = row * a.D;
     // this row, 16-bit values kept as they are until they are used
     const Raw rc = rr, dc = dr, hc = hr, gc = gr;
@@ -479,8 +499,8 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
       w2.get(col, w);
 #pragma unroll
       for (int e = 0; e < EPT; ++e) {
-        const float g = on ? hc[e] : 0.f;  // no row, no part in the sums
-        acc[kP1][e] += on ? g * sh[e] : 0.f;
+        const float g = hc[e];
+        acc[kP1][e] += g * sh[e];
         acc[kP0][e] += g;
         gh[e] = g * w[e];
         p += col.own(e) ? gh[e] : 0.f;
@@ -491,10 +511,10 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
       q *= inv_d;
 #pragma unroll
       for (int e = 0; e < EPT; ++e)
-        ds[e] = (on ? dc[e] : 0.f) + r2 * (gh[e] - p - sh[e] * q);
+        ds[e] = dc[e] + r2 * (gh[e] - p - sh[e] * q);
     } else {
 #pragma unroll
-      for (int e = 0; e < EPT; ++e) ds[e] = on ? dc[e] : 0.f;
+      for (int e = 0; e < EPT; ++e) ds[e] = dc[e];
     }
     float p = 0.f, q = 0.f, dr_[EPT];
     gates();
@@ -509,9 +529,9 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
       ds[e] = cb * d;    // and of u
       if constexpr (is_channel(GATE) || POST) {
         const float t = is_channel(GATE) ? d : ds[e];
-        acc[kS1][e] += on ? t * x[e] : 0.f;
-        acc[kS0][e] += on ? t : 0.f;
-        if constexpr (GATE == kHighCh) acc[kS2][e] += on ? d * rc[e] : 0.f;
+        acc[kS1][e] += t * x[e];
+        acc[kS0][e] += t;
+        if constexpr (GATE == kHighCh) acc[kS2][e] += d * rc[e];
       }
       if constexpr (is_token(GATE)) {
         const float u = POST ? x[e] * w[e] + bb[e] : x[e];
@@ -551,7 +571,7 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
 #pragma unroll
       for (int e = 0; e < EPT; ++e)
         if (col.own(e)) out[col.at[e / VEC] + e % VEC] = acc[p][e];
-    } else {  // blockDim.x is 256 here
+    } else {  // blockDim.x is 256
       __syncthreads();
 #pragma unroll
       for (int e = 0; e < EPT; ++e)
@@ -602,6 +622,7 @@ struct NormPlan {
   else if (pl.place == kWave && pl.ept == 8) {                            \
     SIDES(T, V, 8, kWave, 256, FN)                                        \
   } else if (pl.place == kWave) { SIDES(T, V, 16, kWave, 256, FN) }       \
+  else if (pl.place == kPair) { SIDES(T, V, 8, kPair, 256, FN) }          \
   else if (pl.ept == 8) { SIDES(T, V, 8, kBlock, 512, FN) }               \
   else if (pl.threads <= 512) { SIDES(T, V, 16, kBlock, 512, FN) }        \
   else { SIDES(T, V, 16, kBlock, 1024, FN) }
