@@ -524,7 +524,8 @@ class TransformerModel(nn.Module):
                 attn(f"decoder_l{i}_context", layer.context_attn,
                      layer.post_ctx)
             ffn(f"decoder_l{i}_ffn", layer.ffn, layer.post_ffn)
-            pre_items(f"decoder_l{i}_self_Wq", layer.pre_self)
+            pre_items(f"decoder_l{i}_rnn" if layer.autoreg == "rnn"
+                      else f"decoder_l{i}_self_Wq", layer.pre_self)
             pre_items(f"decoder_l{i}_context_Wq", layer.pre_ctx)
             pre_items(f"decoder_l{i}_ffn_W1", layer.pre_ffn)
         if self.post_top_enc is not None:

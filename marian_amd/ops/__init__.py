@@ -290,8 +290,8 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor,
         f_t = sigmoid(gate_t);  c_t = f_t c_{t-1} + (1 - f_t) x_t
         y_t = act(c_t)          act: "none" | "relu"
 
-    x, gate: [B, T, D], fp32 / bf16 / fp16, any batch and time strides (the
-    last dimension is copied if it is not dense). state: float32 [B, D], the
+    x, gate: [B, T, D], fp32 / bf16 / fp16, D < 2^25, any batch and time
+    strides (copied if the last dimension is not dense). state: float32 [B, D], the
     state before the first step (default zeros). lens: int32 [B]; the steps
     of row b are its first lens[b] positions (clamped to 0..T); what lies
     behind them is ignored, y is 0 there and so are its gradients.
@@ -331,8 +331,9 @@ def gated_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor,
     """One step of gated_scan for each row; returns (y, new_state).
 
     x, gate: [N, D] (rows may be strided); state: float32 [N, D]. inplace
-    writes the new state over `state` (which must be dense) and returns it,
-    as a captured decode step needs; that call has no gradient. Otherwise a
+    writes the new state over `state` (which must be dense and share no
+    memory with x or gate) and returns it, as a captured decode step needs;
+    that call has no gradient. Otherwise a
     call that needs gradients runs as gated_scan over one position.
     """
     if _on_gpu(x):
@@ -347,6 +348,11 @@ def gated_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor,
             raise ValueError("gated_step: inplace has no gradient")
         if not state.is_contiguous():
             raise ValueError("gated_step: inplace needs a dense state")
+        own = state.untyped_storage().data_ptr()
+        if own in (x.untyped_storage().data_ptr(),
+                   gate.untyped_storage().data_ptr()):
+            raise ValueError("gated_step: inplace needs a state of its own "
+                             "memory")
     y, new = gated_scan_torch(x[:, None], gate[:, None], state, act=act)
     return y[:, 0], state.copy_(new) if inplace else new
 

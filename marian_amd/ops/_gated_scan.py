@@ -21,8 +21,9 @@ def check_scan(what, x, gate, state, lens, act, dims):
                          f"shape {tuple(x.shape)}")
     if gate.dtype != x.dtype or gate.device != x.device:
         raise ValueError(f"{what}: x and gate must share dtype and device")
-    if x.shape[-1] == 0:
-        raise ValueError(f"{what}: the width must be positive")
+    if not 0 < x.shape[-1] < 1 << 25:
+        raise ValueError(f"{what}: the width must be 1..2^25-1, got "
+                         f"{x.shape[-1]}")
     if x.dtype not in _DTYPES:
         raise ValueError(f"{what}: unsupported dtype {x.dtype}")
     if act not in _ACTS:

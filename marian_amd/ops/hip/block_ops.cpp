@@ -76,7 +76,9 @@ void check_scan(const char* what, const Tensor& x, const Tensor& gate,
   REFUSE_UNLESS(gate.scalar_type() == x.scalar_type() &&
                     gate.device() == x.device(),
                 what, ": x and gate must share dtype and device");
-  REFUSE_UNLESS(x.size(-1) > 0, what, ": the width must be positive");
+  // a fused projection's rows are twice as wide; lane offsets reach 2^26
+  REFUSE_UNLESS(x.size(-1) > 0 && x.size(-1) < (1L << 25), what,
+                ": the width must be 1..2^25-1, got ", x.size(-1));
   REFUSE_UNLESS(dtype_ok(x), what, ": unsupported dtype ", x.scalar_type());
   if (state.defined())
     REFUSE_UNLESS(state.dim() == 2 && state.size(0) == x.size(0) &&
@@ -255,6 +257,8 @@ std::tuple<Tensor, Tensor> gated_step(Tensor x, Tensor gate, OptTensor state_,
     REFUSE_UNLESS(!grad, "gated_step: inplace has no gradient");
     REFUSE_UNLESS(state.is_contiguous(),
                   "gated_step: inplace needs a dense state");
+    REFUSE_UNLESS(!state.is_alias_of(x) && !state.is_alias_of(gate),
+                  "gated_step: inplace needs a state of its own memory");
   } else if (grad) {
     auto out = scan(x.unsqueeze(1), gate.unsqueeze(1), state, Tensor(), false,
                     relu);
@@ -262,8 +266,10 @@ std::tuple<Tensor, Tensor> gated_step(Tensor x, Tensor gate, OptTensor state_,
   }
   state = state.contiguous();
   Tensor out = inplace ? state : mamd::fresh_like(state);
-  return {gated_step_fwd(dense_rows(x), dense_rows(gate), state, out, relu),
-          out};
+  Tensor y = gated_step_fwd(dense_rows(x), dense_rows(gate), state, out, relu);
+  // a graph that saved the old state must notice
+  if (inplace && !state.is_inference()) torch::autograd::impl::bump_version(state);
+  return {y, out};
 }
 
 std::tuple<Tensor, OptTensor> block_norm(

@@ -398,3 +398,18 @@ def test_gpu_captured():
             graph.replay()
         for _, outs, once in graphs:
             assert all(torch.equal(p, q) for p, q in zip(outs, once()))
+
+
+@pytest.mark.gpu
+def test_gpu_offsets_beyond_32_bits():
+    """More than 2^31 elements: the last rows come out as they do on their
+    own, gradients too."""
+    R, n, D = 4_400_000, 1000, 512
+    t = make(n, D, torch.bfloat16, "cuda", gate="scale", per_token=True)
+    big = {k: v.repeat(R // n, 1) if v is not None and v.dim() == 2 else v
+           for k, v in t.items()}
+    s, h, g = run(big, "layer", "scale", 0.5)
+    s2, h2, g2 = run(t, "layer", "scale", 0.5)
+    assert torch.equal(s[-n:], s2) and torch.equal(h[-n:], h2)
+    for k in ("x", "res", "gate"):
+        assert torch.equal(g[k][-n:], g2[k]), k

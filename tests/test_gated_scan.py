@@ -228,7 +228,21 @@ def test_step_refusals(dev):
     _refused(ops.gated_step, x, x, s.half())
     _refused(ops.gated_step, x, x, torch.zeros(4, 2, device=dev).t(),
              inplace=True)
+    _refused(ops.gated_step, x, s, s, inplace=True)
     _refused(ops.gated_step, x.requires_grad_(), x, s, inplace=True)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_step_in_place_is_seen_by_autograd(dev):
+    """A graph that holds the old state does not use the new one."""
+    x = torch.randn(2, 4, device=dev, requires_grad=True)
+    s = torch.randn(2, 4, device=dev)
+    y, _ = ops.gated_step(x, x, s)
+    with torch.no_grad():
+        ops.gated_step(x.detach().clone(), x.detach().clone(), s,
+                       inplace=True)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
 
 
 # ------------------------------------------------------------------ on the GPU
@@ -429,3 +443,32 @@ def test_scan_gpu_captured():
             graph.replay()
         for _, outs, once in graphs:
             assert all(torch.equal(p, q) for p, q in zip(outs, once()))
+
+
+@pytest.mark.gpu
+def test_scan_gpu_offsets_beyond_32_bits():
+    """More than 2^31 elements: the last sequences come out as they do on
+    their own."""
+    B, T, D = 540_000, 64, 64
+    part = torch.randn(1000, T, 2 * D, device="cuda").bfloat16()
+    xg = part.repeat(B // 1000, 1, 1).requires_grad_()
+    st = torch.randn(B, D, device="cuda")
+    dy = torch.randn(1000, T, D, device="cuda").bfloat16()
+    y, last = ops.gated_scan_xg(xg, st, reverse=True)
+    g, = torch.autograd.grad(y, xg, dy.repeat(B // 1000, 1, 1))
+    tail = xg.detach()[-3:].clone().requires_grad_()
+    y2, last2 = ops.gated_scan_xg(tail, st[-3:], reverse=True)
+    g2, = torch.autograd.grad(y2, tail, dy[-3:])
+    assert torch.equal(y[-3:], y2) and torch.equal(last[-3:], last2)
+    assert torch.equal(g[-3:], g2)
+
+
+@pytest.mark.gpu
+def test_step_gpu_offsets_beyond_32_bits():
+    N, D = 2_200_000, 1000
+    part = torch.randn(1000, 2 * D, device="cuda").bfloat16()
+    xg = part.repeat(N // 1000, 1)
+    st = torch.randn(1000, D, device="cuda").repeat(N // 1000, 1)
+    y, new = ops.gated_step(xg[:, :D], xg[:, D:], st, act="relu")
+    y2, new2 = ops.gated_step(part[:, :D], part[:, D:], st[:1000], act="relu")
+    assert torch.equal(y[-1000:], y2) and torch.equal(new[-1000:], new2)

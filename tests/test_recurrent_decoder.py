@@ -78,7 +78,7 @@ TOL = 2.0 ** -12
 
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("post_s", ["dga", "dnga", "drgan", "dh", "dhn", "dra",
-                                    "da", "dan", "gd", "nargh"])
+                                    "da", "dan", "gd", "nargh", "nan", "rar"])
 @pytest.mark.parametrize("pre_s", ["n", "r", ""])
 def test_strings_and_their_gradients(dev, post_s, pre_s):
     torch.manual_seed(3)
