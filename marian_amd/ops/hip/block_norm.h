@@ -26,6 +26,15 @@
 // its rows and adds up their parameter gradients in registers; the blocks'
 // partial rows are summed by a second kernel in a fixed order (no atomics).
 //
+// What bounds it: bytes. 65536 x 1024 bf16 with a channel gate: forward 4
+// tensors in 107 us (5.0 TB/s; a copy of 2 GB runs at 4.9), backward 6 in 173
+// with the parameter sums (4.7). On the way there: parameters and the next
+// row kept in registers and rows walked by as many blocks as the GPU holds at
+// once (250 -> 107 and 393 -> 190 us), two rows a block in the backward pass
+// (-> 173). Rows of 4097 columns on have 16 elements a lane and no registers
+// for the next row (8192 x 8192 backward: 195 us, 4.1 TB/s); from 8193 on the
+// backward pass spills (2048 x 16384: 356 us, 1.1 TB/s).
+//
 // The kernels are instantiated per element type, a source file each.
 #pragma once
 
