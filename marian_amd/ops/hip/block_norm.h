@@ -32,8 +32,11 @@
 // row kept in registers and rows walked by as many blocks as the GPU holds at
 // once (250 -> 107 and 393 -> 190 us), two rows a block in the backward pass
 // (-> 173). Rows of 4097 columns on have 16 elements a lane and no registers
-// for the next row (8192 x 8192 backward: 195 us, 4.1 TB/s); from 8193 on the
-// backward pass spills (2048 x 16384: 356 us, 1.1 TB/s).
+// for the next row in the backward pass, unless the norms are rms without
+// biases, whose kernel has 32 sums fewer to hold; that one is as fast at 2048 x
+// 8192 (bf16 with a gate, whole pass: 78 us) and 178 us for 188 at 8192 x 8192,
+// 77 for 95 at 4096 x 6000. From 8193 columns on the backward pass spills:
+// 342 us at 2048 x 16384, 227 for rms without biases.
 //
 // The kernels are instantiated per element type, a source file each.
 #pragma once
@@ -415,15 +418,19 @@ __global__ __launch_bounds__(MAXT) void join_fwd_kernel(NormArgs a) {
   }
 }
 
+// LEAN: rms norms without biases, which need neither the mean nor the sums of
+// gradients alone.
 template <typename T, int VEC, int EPT, int PLACE, bool POST, bool PRE,
-          int GATE, int MAXT>
+          int GATE, int MAXT, bool LEAN>
 __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
   constexpr int NC = EPT / VEC;
   // blocks of 1024 have 128 registers a lane: parameters are read again for
   // each row and nothing is fetched ahead
   constexpr bool KEEP = MAXT <= 512;
-  // rows of 16 elements a lane leave no registers for the next row's
-  constexpr bool AHEAD = KEEP && !(PLACE == kBlock && EPT == 16);
+  // rows of 16 elements a lane leave no registers for the next row's, except
+  // where the sums are few (4096 x 6000: 75 us for 85); a highway's spill
+  constexpr bool AHEAD = KEEP && (!(PLACE == kBlock && EPT == 16) ||
+                                 (LEAN && !is_highway(GATE)));
   using Raw = RawRow<T, VEC, NC>;
   __shared__ float buf[2][32];
   // the lane groups' sums of one parameter
@@ -434,7 +441,7 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
   const Columns<VEC, NC> col(it.lane, a.tpr, a.D);
   const Param<T, VEC, NC, KEEP> w1(POST ? a.post_scale : nullptr, a.param32, 1.f,
                              col);
-  const Param<T, VEC, NC, KEEP> b1(POST ? a.post_bias : nullptr, a.param32, 0.f,
+  const Param<T, VEC, NC, KEEP> b1(POST && !LEAN ? a.post_bias : nullptr, a.param32, 0.f,
                              col);
   const Param<T, VEC, NC, KEEP> w2(PRE ? a.pre_scale : nullptr, a.param32, 1.f, col);
   const Param<T, VEC, NC, KEEP> gp(is_channel(GATE) ? a.gate : nullptr,
@@ -482,7 +489,8 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
     const long base = row * a.D;
     // this row, 16-bit values kept as they are until they are used
     const Raw rc = rr, dc = dr, hc = hr, gc = gr;
-    const float m1 = st[0], r1 = st[1], m2 = st[2], r2 = st[3];
+    const float m1 = LEAN ? 0.f : st[0], r1 = st[1];
+    const float m2 = LEAN ? 0.f : st[2], r2 = st[3];
     float x[EPT], ds[EPT], w[EPT], bb[EPT], gt[EPT];
 #pragma unroll
     for (int e = 0; e < EPT; ++e)  // the normalised row
@@ -494,9 +502,27 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
       for (int e = 0; e < EPT; ++e)
         if constexpr (!is_channel(GATE)) gt[e] = is_token(GATE) ? gc[e] : 0.f;
     };
+    auto bias = [&](float o[EPT]) __attribute__((always_inline)) {
+      if constexpr (LEAN) {
+#pragma unroll
+        for (int e = 0; e < EPT; ++e) o[e] = 0.f;
+      } else {
+        b1.get(col, o);
+      }
+    };
+    auto row_sums = [&](float& p, float& q) __attribute__((always_inline)) {
+      if constexpr (LEAN) {
+        sum(q);
+        p = 0.f;
+      } else {
+        sum(p, q);
+        p = a.rms ? 0.f : p * inv_d;
+      }
+      q *= inv_d;
+    };
     if constexpr (PRE) {
       float sh[EPT], gh[EPT], p = 0.f, q = 0.f;
-      if constexpr (POST) w1.get(col, w), b1.get(col, bb);
+      if constexpr (POST) w1.get(col, w), bias(bb);
       gates();
 #pragma unroll
       for (int e = 0; e < EPT; ++e) {
@@ -510,14 +536,12 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
       for (int e = 0; e < EPT; ++e) {
         const float g = hc[e];
         acc[kP1][e] += g * sh[e];
-        acc[kP0][e] += g;
+        if (!LEAN) acc[kP0][e] += g;
         gh[e] = g * w[e];
         p += col.own(e) ? gh[e] : 0.f;
         q += col.own(e) ? gh[e] * sh[e] : 0.f;
       }
-      sum(p, q);
-      p = a.rms ? 0.f : p * inv_d;
-      q *= inv_d;
+      row_sums(p, q);
 #pragma unroll
       for (int e = 0; e < EPT; ++e)
         ds[e] = dc[e] + r2 * (gh[e] - p - sh[e] * q);
@@ -528,7 +552,7 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
     float p = 0.f, q = 0.f, dr_[EPT];
     gates();
     if constexpr (POST) w1.get(col, w);
-    if constexpr (POST && is_token(GATE)) b1.get(col, bb);
+    if constexpr (POST && is_token(GATE)) bias(bb);
 #pragma unroll
     for (int e = 0; e < EPT; ++e) {
       float ca, cb, k1;
@@ -539,7 +563,7 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
       if constexpr (is_channel(GATE) || POST) {
         const float t = is_channel(GATE) ? d : ds[e];
         acc[kS1][e] += t * x[e];
-        acc[kS0][e] += t;
+        if (!LEAN) acc[kS0][e] += t;
         if constexpr (GATE == kHighCh) acc[kS2][e] += d * rc[e];
       }
       if constexpr (is_token(GATE)) {
@@ -562,9 +586,7 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
     put(a.dres, dr_);
     if constexpr (is_token(GATE)) put(a.dgate, gt);
     if constexpr (POST) {
-      sum(p, q);
-      p = a.rms ? 0.f : p * inv_d;
-      q *= inv_d;
+      row_sums(p, q);
 #pragma unroll
       for (int e = 0; e < EPT; ++e) ds[e] = r1 * (ds[e] - p - x[e] * q);
     }
@@ -674,9 +696,16 @@ int join_bwd_launch(const NormPlan& pl, unsigned grid, hipStream_t stream) {
 #define RUN(T, VEC, EPT, PLACE, POST, PRE, GATE, MAXT)                       \
   {                                                                          \
     constexpr auto kernel =                                                  \
-        &join_bwd_kernel<T, VEC, EPT, PLACE, POST, PRE, GATE, MAXT>;         \
-    if (grid == 0) return resident<kernel>(pl.threads);                      \
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(pl.threads), 0, stream, a);  \
+        &join_bwd_kernel<T, VEC, EPT, PLACE, POST, PRE, GATE, MAXT, false>;  \
+    constexpr auto lean =                                                    \
+        &join_bwd_kernel<T, VEC, EPT, PLACE, POST, PRE, GATE, MAXT,          \
+                         PLACE == kBlock && EPT == 16>;                      \
+    const bool is_lean = a.rms && !a.post_bias && !a.pre_bias;               \
+    if (grid == 0)                                                           \
+      return is_lean ? resident<lean>(pl.threads)                            \
+                     : resident<kernel>(pl.threads);                         \
+    hipLaunchKernelGGL(is_lean ? lean : kernel, dim3(grid),                  \
+                       dim3(pl.threads), 0, stream, a);                      \
   }
   WIDTHS(T, RUN)
 #undef RUN

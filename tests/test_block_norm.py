@@ -413,3 +413,41 @@ def test_gpu_offsets_beyond_32_bits():
     assert torch.equal(s[-n:], s2) and torch.equal(h[-n:], h2)
     for k in ("x", "res", "gate"):
         assert torch.equal(g[k][-n:], g2[k]), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [
+    dict(R=600, D=4097, dtype=torch.bfloat16, gate="scale", alpha=0.5),
+    dict(R=520, D=9001, dtype=torch.float32),
+    dict(R=3, D=4104, dtype=torch.float16, pdt=torch.float32),
+    dict(R=4, D=6001, dtype=torch.bfloat16, gate="highway"),
+    dict(R=4, D=8192, dtype=torch.bfloat16, gate="scale", per_token=True),
+    dict(R=4, D=8191, dtype=torch.float32, gate="highway", per_token=True),
+    dict(R=4, D=8192, dtype=torch.float32, post=False, gate="scale"),
+    dict(R=4, D=5000, dtype=torch.float16, pre=False),
+    dict(R=3, D=8193, dtype=torch.bfloat16, gate="highway", alpha=0.7),
+    dict(R=3, D=16384, dtype=torch.bfloat16, no_res=True),
+    dict(R=3, D=16384, dtype=torch.float16, pre=False, gate="scale"),
+])
+def test_gpu_wide_rms(case):
+    """rms norms without biases have a backward kernel of their own for wide
+    rows; 520 and 600 rows give a block several."""
+    check_case("cuda", norm="rms", **case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bias", ["post_bias", "pre_bias"])
+def test_gpu_wide_rms_with_a_bias(bias):
+    t = make(300, 4500, torch.float32, "cuda", norm="rms", gate="scale")
+    t[bias] = torch.linspace(-1, 1, 4500, device="cuda")
+    _, _, grads = run(t, "rms", "scale", 1.0)
+    want = oracle_with_bias(t, bias)
+    for k, g in grads.items():
+        close(k, g, want[k], t[k].dtype)
+
+
+def oracle_with_bias(t, bias):
+    """The oracle takes both biases or none: the other one is zero."""
+    zero = torch.zeros(t["x"].shape[-1], device=t["x"].device)
+    return oracle({k: zero if v is None and k.endswith("bias") else v
+                   for k, v in t.items()}, "rms", "scale", 1.0)
