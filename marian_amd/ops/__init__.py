@@ -260,10 +260,10 @@ def block_norm(x: torch.Tensor, res: Optional[torch.Tensor],
 
     norm: "layer" ((v - mean) / sqrt(var + eps)) or "rms" (v / sqrt(mean v^2
     + eps)), times scale, plus bias if there is one. x, res: [..., D], fp32 /
-    bf16 / fp16, D <= 16384; without res its term is left out. gate: [D] (per channel) or x's shape (per
-    token). Parameters are [D], all of x's dtype or all float32. h is taken
+    bf16 / fp16, D <= 16384; without res its term is left out. gate: [D] (per
+    channel) or x's shape (per token). Parameters are [D], all of x's dtype or all float32. h is taken
     from the 32-bit s; s and h are rounded once. Differentiable once in every
-    tensor.
+    tensor; on the GPU neither forward-mode derivatives nor traces are taken.
     """
     if _on_gpu(x):
         return hip_ext(required=True).block_norm(
@@ -298,7 +298,8 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor,
     reverse: the steps run from position lens[b]-1 down to 0.
     y: [B, T, D] in x's dtype; last: float32 [B, D], the state after the last
     step (`state` itself for a row of no steps). States are held in 32 bits.
-    Differentiable once in x, gate and state.
+    Differentiable once in x, gate and state; on the GPU neither forward-mode
+    derivatives nor traces are taken.
     """
     if _on_gpu(x):
         return hip_ext(required=True).gated_scan(x, gate, state, lens,
@@ -334,7 +335,8 @@ def gated_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor,
     writes the new state over `state` (which must be dense and share no
     memory with x or gate) and returns it, as a captured decode step needs;
     that call has no gradient. Otherwise a
-    call that needs gradients runs as gated_scan over one position.
+    call that needs gradients runs as gated_scan over one position. On the GPU
+    neither forward-mode derivatives nor traces are taken.
     """
     if _on_gpu(x):
         return hip_ext(required=True).gated_step(x, gate, state, act, inplace)

@@ -4,6 +4,7 @@
 // step and about 100 us for a training pass, more than the kernels.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "fresh.h"
 
@@ -42,6 +43,17 @@ OptTensor opt(const Tensor& t) {
 }
 Tensor plain(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+// The kernels are called on memory: a tangent would be dropped and a trace
+// would hold the outputs as constants, neither with a word.
+template <typename... Ts>
+void refuse_modes(const char* what, const Ts&... ts) {
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      !((ts.defined() && ts._fw_grad(0).defined()) || ...), what,
+      " has no forward-mode derivative");
+  TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), what,
+                              " cannot be traced on the GPU");
+}
 
 bool dtype_ok(const Tensor& t) {
   const auto s = t.scalar_type();
@@ -229,6 +241,7 @@ struct JoinFn : public torch::autograd::Function<JoinFn> {
 std::tuple<Tensor, Tensor> gated_scan(Tensor x, Tensor gate, OptTensor state,
                                       OptTensor lens, bool reverse,
                                       std::string act) {
+  refuse_modes("gated_scan", x, gate, plain(state));
   check_scan("gated_scan", x, gate, plain(state), plain(lens), 3);
   return scan(x, gate, plain(state), plain(lens), reverse,
               act_relu("gated_scan", act));
@@ -237,6 +250,7 @@ std::tuple<Tensor, Tensor> gated_scan(Tensor x, Tensor gate, OptTensor state,
 std::tuple<Tensor, Tensor> gated_scan_xg(Tensor xg, OptTensor state,
                                          OptTensor lens, bool reverse,
                                          std::string act) {
+  refuse_modes("gated_scan_xg", xg, plain(state));
   REFUSE_UNLESS(xg.dim() == 3 && xg.size(-1) % 2 == 0,
                 "gated_scan_xg: xg must be [B, T, 2D], got ", xg.sizes());
   const Tensor x = half(xg, 0);
@@ -249,6 +263,7 @@ std::tuple<Tensor, Tensor> gated_step(Tensor x, Tensor gate, OptTensor state_,
                                       std::string act, bool inplace) {
   REFUSE_UNLESS(state_.has_value(), "gated_step: state is required");
   Tensor state = *state_;
+  refuse_modes("gated_step", x, gate, state);
   check_scan("gated_step", x, gate, state, Tensor(), 2);
   const bool relu = act_relu("gated_step", act);
   const bool grad = c10::GradMode::is_enabled() &&
@@ -276,6 +291,8 @@ std::tuple<Tensor, OptTensor> block_norm(
     Tensor x, OptTensor res_, OptTensor gate_, std::string gate_kind, double alpha,
     OptTensor post_scale, OptTensor post_bias, OptTensor pre_scale,
     OptTensor pre_bias, std::string norm, double eps) {
+  refuse_modes("block_norm", x, plain(res_), plain(gate_), plain(post_scale),
+               plain(post_bias), plain(pre_scale), plain(pre_bias));
   REFUSE_UNLESS(x.dim() >= 1 && dtype_ok(x),
                 "block_norm: x must be [..., D] in float32, bfloat16 or "
                 "float16, got ", x.scalar_type(), " ", x.sizes());

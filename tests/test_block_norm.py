@@ -236,6 +236,34 @@ def test_refusals(dev):
         refused(x.double(), x.double())
 
 
+@pytest.mark.parametrize("dev", ["cpu", pytest.param(
+    "cuda", marks=pytest.mark.gpu)])
+def test_gpu_call_refuses_modes(dev):
+    """No tangent is dropped and no trace holds a constant. Off the GPU the
+    extension is called, which looks at the mode before it asks for a GPU."""
+    import torch.autograd.forward_ad as fwd
+    ext = ops.hip_ext()
+    if ext is None:
+        pytest.skip("the extension is not built")
+
+    def fn(x, res, gate, w1, b1, w2, b2):
+        if dev == "cuda":
+            return ops.block_norm(x, res, gate, "highway", 0.5, w1, b1, w2, b2)
+        return ext.block_norm(x, res, gate, "highway", 0.5, w1, b1, w2, b2,
+                              "layer", 1e-9)
+    tensors = tuple(torch.randn(2, 3, 4, device=dev) for _ in range(3)) \
+        + tuple(torch.randn(4, device=dev) for _ in range(4))
+    for i, t in enumerate(tensors):
+        for grad in (True, False):
+            with fwd.dual_level(), torch.set_grad_enabled(grad):
+                a = list(tensors)
+                a[i] = fwd.make_dual(t, torch.ones_like(t))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    fn(*a)
+    with torch.no_grad(), pytest.raises(NotImplementedError, match="traced"):
+        torch.jit.trace(fn, tensors, check_trace=False)
+
+
 # ------------------------------------------------------------------ on the GPU
 
 GPU_CASES = [

@@ -245,6 +245,57 @@ def test_step_in_place_is_seen_by_autograd(dev):
         y.sum().backward()
 
 
+def refused_modes(call, *tensors):
+    """No tangent is dropped and no trace holds a constant: each tensor as a
+    dual one, and the call traced."""
+    import torch.autograd.forward_ad as fwd
+    for i, t in enumerate(tensors):
+        for grad in (True, False):
+            with fwd.dual_level(), torch.set_grad_enabled(grad):
+                a = list(tensors)
+                a[i] = fwd.make_dual(t, torch.ones_like(t))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(*a)
+    with torch.no_grad(), pytest.raises(NotImplementedError, match="traced"):
+        torch.jit.trace(call, tensors, check_trace=False)
+
+
+def gpu_entries(dev):
+    """The GPU's entry points; off the GPU the extension's, which look at the
+    mode before they ask for a GPU."""
+    if dev == "cuda":
+        return ops.gated_scan, ops.gated_scan_xg, ops.gated_step
+    ext = ops.hip_ext()
+    if ext is None:
+        pytest.skip("the extension is not built")
+    return (lambda x, g, s: ext.gated_scan(x, g, s, None, False, "none"),
+            lambda xg, s: ext.gated_scan_xg(xg, s, None, False, "none"),
+            lambda x, g, s: ext.gated_step(x, g, s, "none", False))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_gpu_calls_refuse_modes(dev):
+    scan, scan_xg, step = gpu_entries(dev)
+    xg, s = torch.randn(2, 3, 8, device=dev), torch.randn(2, 4, device=dev)
+    refused_modes(lambda x, g, s: scan(x, g, s), xg[..., :4], xg[..., 4:], s)
+    refused_modes(lambda a, s: scan_xg(a, s), xg, s)
+    refused_modes(lambda x, g, s: step(x, g, s), xg[:, 0, :4], xg[:, 0, 4:],
+                  s)
+
+
+def test_forward_mode_off_the_gpu():
+    """There the tangent comes out: against differences."""
+    import torch.autograd.forward_ad as fwd
+    xg, st, ln, _, _ = make(2, 6, 3, torch.float64, "cpu", 3, True, "ragged")
+    v, e = torch.randn_like(xg), 1e-6
+    with fwd.dual_level():
+        y, last = ops.gated_scan_xg(fwd.make_dual(xg, v), st, ln)
+        got = [fwd.unpack_dual(t).tangent for t in (y, last)]
+    up, dn = (ops.gated_scan_xg(xg + k * v, st, ln) for k in (e, -e))
+    for g, a, b in zip(got, up, dn):
+        assert torch.allclose(g, (a - b) / (2 * e), rtol=0, atol=1e-7)
+
+
 # ------------------------------------------------------------------ on the GPU
 
 GPU_CASES = [
