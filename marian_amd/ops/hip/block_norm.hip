@@ -216,9 +216,9 @@ unsigned grid_of(bool bwd, const torch::Tensor& x, const NormPlan& pl,
 }  // namespace
 
 // returns (s, h, stat): h is undefined without pre_scale, stat without
-// want_stat
+// want_stat; s and h have `sizes`, x's before its rows were laid out
 std::vector<torch::Tensor> block_norm_fwd(
-    torch::Tensor x, c10::optional<torch::Tensor> res,
+    at::IntArrayRef sizes, torch::Tensor x, c10::optional<torch::Tensor> res,
     c10::optional<torch::Tensor> gate,
     bool highway, double alpha, c10::optional<torch::Tensor> post_scale,
     c10::optional<torch::Tensor> post_bias,
@@ -229,9 +229,11 @@ std::vector<torch::Tensor> block_norm_fwd(
                       pre_scale, pre_bias, rms, eps, false);
   NormArgs& a = pl.a;
   const c10::DeviceGuard guard(x.device());
-  auto s = fresh_like(x);
+  TORCH_CHECK(c10::multiply_integers(sizes) == x.numel(),
+              "block_norm: sizes are not x's");
+  auto s = fresh(sizes, x.scalar_type(), x);
   torch::Tensor h, stat;
-  if (a.pre_scale) h = fresh_like(x), a.h = h.data_ptr();
+  if (a.pre_scale) h = fresh_like(s), a.h = h.data_ptr();
   if (want_stat) {
     stat = fresh({4, a.rows}, torch::kFloat32, x);
     a.stat = stat.data_ptr<float>();

@@ -21,7 +21,8 @@ Tensor gated_scan_bwd(Tensor x, Tensor gate, OptTensor state, OptTensor lens,
                       bool relu, Tensor dx, Tensor dgate, bool want_dstate);
 Tensor gated_step_fwd(Tensor x, Tensor gate, Tensor state, Tensor state_out,
                       bool relu);
-std::vector<Tensor> block_norm_fwd(Tensor x, OptTensor res, OptTensor gate,
+std::vector<Tensor> block_norm_fwd(at::IntArrayRef sizes, Tensor x,
+                                   OptTensor res, OptTensor gate,
                                    bool highway, double alpha,
                                    OptTensor post_scale, OptTensor post_bias,
                                    OptTensor pre_scale, OptTensor pre_bias,
@@ -198,8 +199,9 @@ struct JoinFn : public torch::autograd::Function<JoinFn> {
                                const OptTensor& w2, const OptTensor& b2,
                                bool channel, bool highway, double alpha,
                                bool rms, double eps) {
-    auto out = block_norm_fwd(rows(x), rows(res, false), rows(gate, channel),
-                              highway, alpha, w1, b1, w2, b2, rms, eps, true);
+    auto out = block_norm_fwd(x.sizes(), rows(x), rows(res, false),
+                              rows(gate, channel), highway, alpha, w1, b1, w2,
+                              b2, rms, eps, true);
     ctx->save_for_backward({x, plain(res), plain(gate), plain(w1), plain(b1),
                             plain(w2), plain(b2), out[2]});
     ctx->saved_data["channel"] = channel;
@@ -208,8 +210,9 @@ struct JoinFn : public torch::autograd::Function<JoinFn> {
     ctx->saved_data["rms"] = rms;
     ctx->saved_data["eps"] = eps;
     ctx->set_materialize_grads(false);
-    if (!w2.has_value()) return {like(out[0], x)};
-    return {like(out[0], x), like(out[1], x)};
+    // not views of rows: a caller may change them in place
+    if (!w2.has_value()) return {out[0]};
+    return {out[0], out[1]};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list g) {
@@ -358,9 +361,9 @@ std::tuple<Tensor, OptTensor> block_norm(
     return {out[0], out.size() > 1 ? OptTensor(out[1]) : OptTensor()};
   }
   const at::NoGradGuard no_grad;
-  auto out = block_norm_fwd(rows(x), rows(opt(res), false), rows(opt(gate), channel_gate),
-                            highway, alpha, opt(vec[0]), opt(vec[1]),
-                            opt(vec[2]), opt(vec[3]), rms, eps, false);
-  return {like(out[0], x),
-          vec[2].defined() ? OptTensor(like(out[1], x)) : OptTensor()};
+  auto out = block_norm_fwd(x.sizes(), rows(x), rows(opt(res), false),
+                            rows(opt(gate), channel_gate), highway, alpha,
+                            opt(vec[0]), opt(vec[1]), opt(vec[2]), opt(vec[3]),
+                            rms, eps, false);
+  return {out[0], opt(out[1])};
 }

@@ -264,6 +264,41 @@ def test_gpu_call_refuses_modes(dev):
         torch.jit.trace(fn, tensors, check_trace=False)
 
 
+@pytest.mark.parametrize("dev", ["cpu", pytest.param(
+    "cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("pre", [True, False])
+@pytest.mark.parametrize("lead", [(6,), (2, 3), (2, 1, 3)])
+def test_outputs_may_be_changed_in_place(dev, lead, pre):
+    """As a following in-place op does, whatever the number of dimensions:
+    with a gradient of its own, and where only what changes them has one."""
+    t = make(6, 40, torch.float32, dev, gate="scale", pre=pre)
+    v = {k: a.view(*lead, 40) if a is not None and a.dim() == 2 else a
+         for k, a in t.items()}
+    leaves = [v[k] for k in LEAVES if v[k] is not None]
+    c = torch.full_like(v["x"], 1.5)
+    changed = lambda o, c: o.mul_(c).relu_()
+
+    outs = [o for o in call(v, "layer", "scale", 0.5) if o is not None]
+    for o in outs:              # no gradient but c's
+        got = changed(o.clone(), c)
+        cg = c.clone().requires_grad_()
+        now = changed(o, cg)
+        assert torch.equal(now, got)
+        g, = torch.autograd.grad(now.sum(), cg)
+        assert torch.equal(g != 0, now > 0)
+    for a in leaves:
+        a.requires_grad_()
+
+    def grads(fn):
+        outs = [o for o in call(v, "layer", "scale", 0.5) if o is not None]
+        outs = [fn(o) for o in outs]
+        return outs + list(torch.autograd.grad(
+            outs, leaves, [torch.ones_like(o) for o in outs]))
+    for p, q in zip(grads(lambda o: changed(o, c)),
+                    grads(lambda o: changed(o.clone(), c))):
+        assert torch.equal(p, q)
+
+
 # ------------------------------------------------------------------ on the GPU
 
 GPU_CASES = [

@@ -296,6 +296,24 @@ def test_forward_mode_off_the_gpu():
         assert torch.allclose(g, (a - b) / (2 * e), rtol=0, atol=1e-7)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_outputs_may_be_changed_in_place(dev):
+    xg, st, _, _, _ = make(2, 5, 6, torch.float32, dev, 3)
+    xg.requires_grad_(), st.requires_grad_()
+    calls = [lambda: ops.gated_scan_xg(xg, st),
+             lambda: ops.gated_scan(xg[..., :6], xg[..., 6:], st),
+             lambda: ops.gated_step(xg[:, 0, :6], xg[:, 0, 6:], st)]
+    for fn in calls:
+        res = []
+        for copy in (False, True):
+            outs = [o.clone() if copy else o for o in fn()]
+            for o in outs:
+                o.mul_(1.5).relu_()
+            res.append(outs + list(torch.autograd.grad(
+                outs, (xg, st), [torch.ones_like(o) for o in outs])))
+        assert all(torch.equal(p, q) for p, q in zip(*res))
+
+
 # ------------------------------------------------------------------ on the GPU
 
 GPU_CASES = [
