@@ -56,6 +56,40 @@ def check_join(x, res, gate, gate_kind, params, norm):
             raise ValueError(f"block_norm: {k} must be [{D}] on x's device")
 
 
+def _highway(u, r, g):
+    return torch.sigmoid(-g) * r + torch.sigmoid(g) * u
+
+
+class _Highway(torch.autograd.Function):
+    """(1 - k) r + k u, k = sigmoid(g), whose gate's gradient is made of u - r:
+    the sums of u ds and of r ds, which differentiating the formula gives,
+    cancel where u and r have a common mean."""
+
+    @staticmethod
+    def forward(u, r, g):
+        return _highway(u, r, g)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.save_for_backward(*inputs)
+        ctx.save_for_forward(*inputs)
+
+    @staticmethod
+    def backward(ctx, d):
+        u, r, g = ctx.saved_tensors
+        k, k1 = torch.sigmoid(g), torch.sigmoid(-g)
+        return k * d, k1 * d, (k * k1 * ((u - r) * d)).sum_to_size(g.shape)
+
+    @staticmethod
+    def jvp(ctx, du, dr, dg):
+        u, r, g = ctx.saved_tensors
+        k, k1 = torch.sigmoid(g), torch.sigmoid(-g)
+        out = torch.zeros_like(u)
+        for coef, t in ((k, du), (k1, dr), (k * k1 * (u - r), dg)):
+            out = out if t is None else out + coef * t
+        return out
+
+
 def block_norm_torch(x, res, gate=None, gate_kind="scale", res_scale=1.0,
                      post_scale=None, post_bias=None, pre_scale=None,
                      pre_bias=None, norm="layer", eps=1e-9):
@@ -77,8 +111,9 @@ def block_norm_torch(x, res, gate=None, gate_kind="scale", res_scale=1.0,
     elif gate_kind == "scale":
         s = r + gate.to(acc) * u
     else:
-        g = gate.to(acc)
-        s = torch.sigmoid(-g) * r + torch.sigmoid(g) * u
+        # a trace (model export) takes the formula's own ops
+        highway = _highway if torch.jit.is_tracing() else _Highway.apply
+        s = highway(u, r, gate.to(acc))
     h = None if pre_scale is None else normed(s, pre_scale, pre_bias).to(
         x.dtype)
     return s.to(x.dtype), h

@@ -30,7 +30,6 @@ struct SumArgs {
   int n, D;
   int slot[kNumSums];
   int gate;                  // kNone unless the gate is per channel
-  float alpha;
   const void* gate_p;        // parameters as in NormArgs
   const void* w1;
   const void* b1;
@@ -76,13 +75,13 @@ __global__ __launch_bounds__(1024) void param_sum_kernel(SumArgs a) {
   float b = 1.f, dg = 0.f;
   if (a.gate != kNone) {
     const float g = (float)((const P*)a.gate_p)[c];
-    dg = w1 * s1 + b1 * s0;
     if (a.gate == kHighCh) {
       float k1;
       sigmoid2<float>(g, b, k1);
-      dg = b * k1 * (dg - a.alpha * sum[kS2]);
+      dg = b * k1 * sum[kS2];
     } else {
       b = g;
+      dg = w1 * s1 + b1 * s0;
     }
   }
   const float o[kNumSums] = {dg, b * s1, b * s0, sum[kP1], sum[kP0]};
@@ -293,7 +292,8 @@ std::vector<torch::Tensor> block_norm_bwd(
   const bool dg = vec(2, channel), dw1 = vec(3, a.post_scale),
              db1 = vec(4, a.post_bias), dw2 = vec(5, a.pre_scale),
              db2 = vec(6, a.pre_bias);
-  const bool use[kNumSums] = {dw1 || dg, db1 || (dg && a.post_bias),
+  const bool dfac = dg && pl.gate == kScaleCh;
+  const bool use[kNumSums] = {dw1 || dfac, db1 || (dfac && a.post_bias),
                               dg && pl.gate == kHighCh, dw2, db2};
   for (int p = 0; p < kNumSums; ++p)
     sm.slot[p] = a.slot[p] = use[p] ? a.n_part++ : -1;
@@ -315,7 +315,6 @@ std::vector<torch::Tensor> block_norm_bwd(
     sm.part = a.part;
     sm.n = grid, sm.D = a.D;
     sm.gate = channel ? pl.gate : kNone;
-    sm.alpha = a.alpha;
     sm.gate_p = a.gate, sm.w1 = a.post_scale, sm.b1 = a.post_bias;
     const unsigned sgrid = (unsigned)((a.D + 15) / 16);
     auto stream = at::cuda::getCurrentHIPStream();

@@ -264,6 +264,26 @@ def test_gpu_call_refuses_modes(dev):
         torch.jit.trace(fn, tensors, check_trace=False)
 
 
+@pytest.mark.parametrize("gate", ["scale", "highway"])
+@pytest.mark.parametrize("per_token", [True, False])
+def test_plain_other_derivatives(gate, per_token):
+    """Off the GPU: forward mode, second derivatives, traces."""
+    t = make(3, 6, torch.float64, "cpu", gate=gate, per_token=per_token,
+             seed=2)
+    keys = [k for k in LEAVES if t[k] is not None]
+
+    def fn(*a):
+        return call({**t, **dict(zip(keys, a))}, "layer", gate, 0.7)
+    leaves = [t[k].clone().requires_grad_() for k in keys]
+    assert torch.autograd.gradcheck(fn, leaves, check_forward_ad=True)
+    assert torch.autograd.gradgradcheck(fn, leaves)
+    plain = [t[k] for k in keys]
+    traced = torch.jit.trace(fn, plain, check_trace=False)
+    other = [2 * v for v in plain]
+    for a, b in zip(traced(*other), fn(*other)):
+        assert torch.allclose(a, b, rtol=1e-12, atol=1e-12)
+
+
 @pytest.mark.parametrize("dev", ["cpu", pytest.param(
     "cuda", marks=pytest.mark.gpu)])
 @pytest.mark.parametrize("pre", [True, False])
@@ -476,6 +496,33 @@ def test_gpu_offsets_beyond_32_bits():
     assert torch.equal(s[-n:], s2) and torch.equal(h[-n:], h2)
     for k in ("x", "res", "gate"):
         assert torch.equal(g[k][-n:], g2[k]), k
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param(
+    "cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("R,D", [(3000, 3), (3000, 40), (2000, 700),
+                                 (600, 1500), (300, 4100), (40, 8200)])
+@pytest.mark.parametrize("mean", [0.0, 300.0])
+def test_highway_gate_beside_a_common_mean(dev, mean, R, D):
+    """The gate of a channel's highway gets the sum of (x - res) ds, however
+    far from 0 both of them are. Without norms and with a factor of 1, x - res
+    is rounded once, its product with ds once, and the sum over rows stays
+    within 128 u of the sum of absolute values; the sigmoid's parts are good to
+    3 u each and three products follow."""
+    gen = torch.Generator().manual_seed(5)
+    res = torch.randn(R, D, generator=gen) + mean
+    x = res + 0.01 * torch.randn(R, D, generator=gen)
+    ds = torch.randn(R, D, generator=gen) + 0.5
+    gate = torch.randn(D, generator=gen)
+    g = gate.to(dev).requires_grad_()
+    s, _ = ops.block_norm(x.to(dev), res.to(dev), g, "highway")
+    got, = torch.autograd.grad(s, g, ds.to(dev))
+    k = torch.sigmoid(gate.double())
+    terms = (x.double() - res.double()) * ds.double()
+    want = k * (1 - k) * terms.sum(0)
+    lim = (128 + 2 + 6 + 3) * U * k * (1 - k) * terms.abs().sum(0)
+    err = (got.double().cpu() - want).abs()
+    assert bool((err <= lim + U * want.abs()).all()), float((err / lim).max())
 
 
 @pytest.mark.gpu
