@@ -57,13 +57,14 @@ constexpr bool is_token(int g) { return g == kScaleTok || g == kHighTok; }
 // Sums over rows that the parameter gradients are made of, xh and sh the
 // normalised rows (xh = x without a post norm):
 //   dpre_scale = P1, dpre_bias = P0, dpost_scale = b S1, dpost_bias = b S0,
-//   dgate = w1 S1 + b1 S0   (scale, per channel)
-//           k (1-k) S2      (highway, per channel)
-// since b, w1 and b1 do not change along the rows; so a channel's factor costs
-// no accumulators of its own. S2 is the sum of (u - alpha res) ds: made of
-// whole sums of u ds and res ds it would cancel where u and res have a common
-// mean (4096 rows of deviation 1 around 300: 1e-3 of it was wrong, now 1e-7).
-// With a gate per token S1 and S0 take b inside.
+//   dgate = S2, or w1 S1 without a post bias   (scale, per channel)
+//           k (1-k) S2                         (highway, per channel)
+// since b and w1 do not change along the rows. S2 is the sum of u ds, or of
+// (u - alpha res) ds: whole sums of xh ds, ds and res ds, put together
+// afterwards, cancel where a bias takes back a channel that the norm makes
+// large (1 - 3 % of the gradient was wrong, now 0.08 %), or where u and res
+// have a common mean (4096 rows of deviation 1 around 300: 1e-3 of it, now
+// 2e-7). With a gate per token S1 and S0 take b inside.
 enum { kS1 = 0, kS0, kS2, kP1, kP0, kNumSums };
 
 struct NormArgs {
@@ -451,6 +452,22 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
                              a.param32, 0.f, col);
   // s and u are needed by the next norm and by the gate
   constexpr bool NEED = PRE || GATE != kNone;
+  // A factor's S2 takes a fifth sum and its operands, and the registers for a
+  // third wave on each SIMD. In LDS, each lane's to itself, and apart from the
+  // rest of a row (nothing is moved over the two barriers) it leaves them:
+  // whole passes of 131072 x 512 bf16 281 us for 311, 262144 x 200 282 for 329;
+  // where 16 elements a lane spill, 2048 x 8192 117 for 127 and 2048 x 16384
+  // 462 for 552. Rows over two waves (164 registers, 3 waves) and blocks of 8
+  // elements a lane are better off with registers: 65536 x 1024 283 for 291,
+  // 8192 x 4096 174 for 183.
+  constexpr bool FACTOR = GATE == kScaleCh && POST && !LEAN;
+  constexpr bool IN_LDS = FACTOR && (PLACE <= kWave || EPT == 16);
+  constexpr int QUAD = EPT % 4 == 0 ? 4 : 1;
+  __shared__ vec_t<float, QUAD> factor[IN_LDS ? EPT / QUAD * MAXT : 1];
+  if constexpr (IN_LDS) {
+#pragma unroll
+    for (int i = 0; i < EPT / QUAD; ++i) factor[i * MAXT + threadIdx.x] = {};
+  }
 
   float acc[kNumSums][EPT];  // the unused ones are optimised out
 #pragma unroll
@@ -552,11 +569,23 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
 #pragma unroll
       for (int e = 0; e < EPT; ++e) ds[e] = dc[e];
     }
+    if constexpr (IN_LDS) {
+      __builtin_amdgcn_sched_barrier(0);
+      w1.get(col, w);
+      bias(bb);
+#pragma unroll
+      for (int e = 0; e < EPT; ++e)
+        factor[e / QUAD * MAXT + threadIdx.x][e % QUAD] +=
+            (x[e] * w[e] + bb[e]) * ds[e];
+      __builtin_amdgcn_sched_barrier(0);
+    }
     float p = 0.f, q = 0.f, dr_[EPT];
     gates();
     if constexpr (POST) w1.get(col, w);
-    constexpr bool DIFF = is_token(GATE) || GATE == kHighCh;
-    if constexpr (POST && DIFF) bias(bb);
+    // the terms of the gate's gradient are needed one by one
+    constexpr bool TERM = is_token(GATE) || GATE == kHighCh ||
+                          (FACTOR && !IN_LDS);
+    if constexpr (POST && TERM) bias(bb);
 #pragma unroll
     for (int e = 0; e < EPT; ++e) {
       float ca, cb, k1;
@@ -569,10 +598,10 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
         acc[kS1][e] += t * x[e];
         if (!LEAN) acc[kS0][e] += t;
       }
-      if constexpr (DIFF) {
+      if constexpr (TERM) {
         const float u = POST ? x[e] * w[e] + bb[e] : x[e];
         const float du = is_highway(GATE) ? u - a.alpha * rc[e] : u;
-        if constexpr (GATE == kHighCh) acc[kS2][e] += du * d;
+        if constexpr (is_channel(GATE)) acc[kS2][e] += du * d;
         else gt[e] = (is_highway(GATE) ? cb * k1 * du : du) * d;
       }
       if constexpr (POST) {
@@ -598,6 +627,11 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
     put(a.dx, ds);
   }
   if (!a.part) return;
+  if constexpr (IN_LDS) {
+#pragma unroll
+    for (int e = 0; e < EPT; ++e)
+      acc[kS2][e] = factor[e / QUAD * MAXT + threadIdx.x][e % QUAD];
+  }
   float* part = a.part + (size_t)blockIdx.x * a.n_part * a.D;
 #pragma unroll
   for (int p = 0; p < kNumSums; ++p) {

@@ -32,7 +32,6 @@ struct SumArgs {
   int gate;                  // kNone unless the gate is per channel
   const void* gate_p;        // parameters as in NormArgs
   const void* w1;
-  const void* b1;
   void* out[kNumSums];       // dgate, dpost_scale, .._bias, dpre_scale, .._bias
 };
 
@@ -71,7 +70,6 @@ __global__ __launch_bounds__(1024) void param_sum_kernel(SumArgs a) {
     sum[p] = a.slot[p] >= 0 ? total[a.slot[p]][lane] : 0.f;
   const float s1 = sum[kS1], s0 = sum[kS0];
   const float w1 = a.w1 ? (float)((const P*)a.w1)[c] : 1.f;
-  const float b1 = a.b1 ? (float)((const P*)a.b1)[c] : 0.f;
   float b = 1.f, dg = 0.f;
   if (a.gate != kNone) {
     const float g = (float)((const P*)a.gate_p)[c];
@@ -81,7 +79,7 @@ __global__ __launch_bounds__(1024) void param_sum_kernel(SumArgs a) {
       dg = b * k1 * sum[kS2];
     } else {
       b = g;
-      dg = w1 * s1 + b1 * s0;
+      dg = a.slot[kS2] >= 0 ? sum[kS2] : w1 * s1;
     }
   }
   const float o[kNumSums] = {dg, b * s1, b * s0, sum[kP1], sum[kP0]};
@@ -292,9 +290,9 @@ std::vector<torch::Tensor> block_norm_bwd(
   const bool dg = vec(2, channel), dw1 = vec(3, a.post_scale),
              db1 = vec(4, a.post_bias), dw2 = vec(5, a.pre_scale),
              db2 = vec(6, a.pre_bias);
-  const bool dfac = dg && pl.gate == kScaleCh;
-  const bool use[kNumSums] = {dw1 || dfac, db1 || (dfac && a.post_bias),
-                              dg && pl.gate == kHighCh, dw2, db2};
+  const bool terms = pl.gate == kHighCh || a.post_bias;
+  const bool use[kNumSums] = {dw1 || (dg && !terms), db1, dg && terms, dw2,
+                              db2};
   for (int p = 0; p < kNumSums; ++p)
     sm.slot[p] = a.slot[p] = use[p] ? a.n_part++ : -1;
   if (a.rows == 0) {
@@ -315,7 +313,7 @@ std::vector<torch::Tensor> block_norm_bwd(
     sm.part = a.part;
     sm.n = grid, sm.D = a.D;
     sm.gate = channel ? pl.gate : kNone;
-    sm.gate_p = a.gate, sm.w1 = a.post_scale, sm.b1 = a.post_bias;
+    sm.gate_p = a.gate, sm.w1 = a.post_scale;
     const unsigned sgrid = (unsigned)((a.D + 15) / 16);
     auto stream = at::cuda::getCurrentHIPStream();
 #define SUMN(P, NP)                                                          \

@@ -525,6 +525,34 @@ def test_highway_gate_beside_a_common_mean(dev, mean, R, D):
     assert bool((err <= lim + U * want.abs()).all()), float((err / lim).max())
 
 
+@pytest.mark.parametrize("dev", ["cpu", pytest.param(
+    "cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("R,D", [(4096, 2), (4096, 64), (3000, 256),
+                                 (3000, 512), (3000, 1024), (1500, 2048),
+                                 (600, 8192), (600, 16384)])
+def test_factor_behind_a_cancelled_channel(dev, R, D):
+    """The factor of a channel whose bias takes back what the norm makes of it
+    gets the sum of u ds. Rows of 1 and -1 have a root mean square of 1 exactly
+    (D is a power of two, eps vanishes beside 1), so a channel of ones with
+    the bias -1 + 2^-16 has u = 2^-16 exactly; the product with ds is rounded
+    once and the sum over rows stays within 128 u of the sum of absolute
+    values. The sums of xh ds and of ds themselves are 2^16 times as large."""
+    gen = torch.Generator().manual_seed(6)
+    x = torch.randint(0, 2, (R, D), generator=gen).float() * 2 - 1
+    x[:, 1] = 1
+    ds = torch.randn(R, D, generator=gen) + 0.5
+    w, b = torch.ones(D), torch.zeros(D)
+    b[1] = -1 + 2.0 ** -16
+    g = torch.ones(D).to(dev).requires_grad_()
+    s, _ = ops.block_norm(x.to(dev), None, g, post_scale=w.to(dev),
+                          post_bias=b.to(dev), norm="rms", eps=1e-30)
+    got, = torch.autograd.grad(s, g, ds.to(dev))
+    terms = (x.double() + b.double()) * ds.double()
+    err = (got.double().cpu() - terms.sum(0)).abs()
+    lim = 130 * U * terms.abs().sum(0)
+    assert bool((err <= lim).all()), float((err / lim).max())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("case", [
     dict(R=600, D=4097, dtype=torch.bfloat16, gate="scale", alpha=0.5),
