@@ -18,6 +18,7 @@ import torch
 import torch.nn as nn
 
 from .. import ops
+from ..ops.cpu_int8 import int8_enabled
 
 
 class Dense(nn.Module):
@@ -525,13 +526,16 @@ class SSRU(nn.Module):
         return self.W_xg[:, i * self.dim:(i + 1) * self.dim]
 
     def project(self, x):
-        """[x W, x Wf + bf]; only the gate half has a bias."""
-        if torch.is_grad_enabled():
-            return ops.linear(x, self.W_xg,
-                              torch.nn.functional.pad(self.bf, (self.dim, 0)))
-        xg = ops.linear(x, self.W_xg)   # packed int8 weights stay cached
-        xg[..., self.dim:] += self.bf.to(xg.dtype)
-        return xg
+        """[x W, x Wf + bf]; only the gate half has a bias, which the product
+        adds before it is rounded, with gradients and without."""
+        if int8_enabled() and not x.is_cuda and not torch.is_grad_enabled():
+            # weights are packed once for a bias's address: without this one,
+            # which is new for each call; the sum is in float32
+            xg = ops.linear(x, self.W_xg)
+            xg[..., self.dim:] += self.bf.to(xg.dtype)
+            return xg
+        return ops.linear(x, self.W_xg,
+                          torch.nn.functional.pad(self.bf, (self.dim, 0)))
 
     def step(self, x, state, inplace: bool = False):
         """x [N, d], state float32 [N, d] -> (h [N, d], new state)."""

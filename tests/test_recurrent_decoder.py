@@ -10,7 +10,7 @@ from marian_amd.common.config_parser import ConfigParser, MODE_TRAINING
 from marian_amd.common.options import Options
 from marian_amd.data.batch import CorpusBatch, SubBatch
 from marian_amd.data.synthetic import synthetic_batch
-from marian_amd.models.layers import PrePostProcessor, join_blocks
+from marian_amd.models.layers import PrePostProcessor, SSRU, join_blocks
 from marian_amd.models.model_factory import create_model
 from marian_amd.translator.beam_search import BeamSearch, ModelScorer
 
@@ -186,6 +186,54 @@ def test_beam_search():
                      normalize=0.6, max_length=10).search(
                          sentences(), torch.device("cpu"))
     assert len(res) == 3 and all(r.best.tokens for r in res)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("params", ["own", "float32"])
+def test_projection_is_rounded_once(dev, dtype, params):
+    """Scoring and decoding take the projection that training takes: the
+    gate's bias is added before the only rounding. An error of the 32-bit sum
+    over d products is below d + 2 units of the sum of absolute values."""
+    torch.manual_seed(14)
+    cell = SSRU(64)
+    with torch.no_grad():
+        cell.bf.uniform_(-3, 3)
+    if params == "own":
+        cell = cell.to(dtype)
+    cell = cell.to(dev)
+    x = torch.randn(5, 7, 64).to(dtype).to(dev)
+    with_grad = cell.project(x).detach()
+    with torch.no_grad():
+        got = cell.project(x)
+    assert got.dtype == dtype and torch.equal(got, with_grad)
+    W, bf = (p.detach().to(dtype).double().cpu() for p in (cell.W_xg, cell.bf))
+    b = torch.cat([torch.zeros(64, dtype=torch.float64), bf])
+    xd = x.double().cpu()
+    want, size = xd @ W + b, xd.abs() @ W.abs() + b.abs()
+    lim = 66 * 2.0 ** -24 * size
+    half = torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -7)
+    assert bool(((got.double().cpu() - want).abs()
+                 <= lim + half * (want.abs() + lim)).all())
+
+
+def test_projection_with_int8_weights():
+    """Weights are packed once, and the bias is there."""
+    from marian_amd.ops import cpu_int8
+    torch.manual_seed(15)
+    cell, x = SSRU(64), torch.randn(9, 64)
+    with torch.no_grad():
+        cell.bf.uniform_(-3, 3)
+        want = cell.project(x)
+        cpu_int8.enable_int8(True)
+        try:
+            for _ in range(3):
+                got = cell.project(x)
+                assert len(cpu_int8._qcache) == 1
+        finally:
+            cpu_int8.enable_int8(False)
+    assert float((got - want).abs().max()) < 0.1
+    assert not torch.equal(got, want)
 
 
 # ------------------------------------------------------------------ on the GPU
