@@ -59,4 +59,6 @@ def gated_scan_torch(x, gate, state=None, lens=None, reverse=False,
             out = torch.where(on, out, torch.zeros_like(out))
         c, ys[t] = new, out
     y = torch.stack(ys, dim=1) if T else om * xa
+    if c is state:      # no step: its value in memory of its own
+        c = c.clone()
     return y.to(x.dtype), c

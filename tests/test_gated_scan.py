@@ -297,6 +297,20 @@ def test_forward_mode_off_the_gpu():
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("T,lens", [(0, None), (3, 0)])
+def test_last_state_has_memory_of_its_own(dev, T, lens):
+    """Without a step the last state is the first one's value, not its
+    memory."""
+    x, st = torch.ones(2, T, 4, device=dev), torch.ones(2, 4, device=dev)
+    ln = None if lens is None else torch.full((2,), lens, dtype=torch.int32,
+                                              device=dev)
+    _, last = ops.gated_scan(x, x, st, ln)
+    assert torch.equal(last, st)
+    last.zero_()
+    assert bool((st == 1).all())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_outputs_may_be_changed_in_place(dev):
     xg, st, _, _, _ = make(2, 5, 6, torch.float32, dev, 3)
     xg.requires_grad_(), st.requires_grad_()
