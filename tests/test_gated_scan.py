@@ -11,6 +11,7 @@ steps stay within K u amax with K = T (4 gmax + 32), amax the largest |x| or
 lam, c - x and f om <= 1/4. The last rounding to the output's type adds
 eps / 2 of the value.
 """
+import numpy as np
 import pytest
 import torch
 
@@ -555,3 +556,191 @@ def test_step_gpu_offsets_beyond_32_bits():
     y, new = ops.gated_step(xg[:, :D], xg[:, D:], st, act="relu")
     y2, new2 = ops.gated_step(part[:, :D], part[:, D:], st[:1000], act="relu")
     assert torch.equal(y[-1000:], y2) and torch.equal(new[-1000:], new2)
+
+
+# ------------------------------------------------- bounds that a gate damps
+# The limits above grow by a whole step's error with every step. These carry
+# the error through the recurrence, element by element, as the gates damp it.
+#
+# In units of u = 2^-24 the sigmoid's exponential e has an error of at most
+# 2 |g| + 3 (its argument's product and log2(e) are rounded, exp2 is good to
+# one unit in the last place), so f, that is 1 / (1 + e) or e / (1 + e), has
+# om (2 |g| + 3) + 4 and om has f (2 |g| + 3) + 4. A state is the sum of terms
+# om x, each multiplied by the f of the steps behind it, however the steps are
+# grouped: a step brings f's error, one rounding of a product and one of a sum
+# to what is there; joining groups of steps brings at most 32 more to a term
+# (5 in its tile, and folding tiles and chunks rounds less often than their
+# steps would). With M the sum of the terms' absolute values:
+#     E' = f (E + (ef + 2) M) + om |x| (eom + 2),   M' = f M + om |x|
+# and a state is within (E + 32 M) u. The gradient's recurrence is the same
+# one. Where relu's side is not certain within the state's bound, dy may be
+# there or not, which is carried on as an absolute error. 2 % are added for
+# products of errors (1e5 roundings are 0.6 %).
+
+JOINS, MORE = 32, 1.02
+
+
+def sharp(x, g, state, lens, reverse, act, dy, dlast, drop=0, states=None):
+    """{name: (value, bound)} in float64, before the last rounding. Mistakes
+    for the checks of the bounds: drop > 0 loses the gradient's carry every
+    `drop` steps, states rounds the state at each 64th step to that type."""
+    B, T, D = x.shape
+    f, om = torch.sigmoid(g.double()), torch.sigmoid(-g.double())
+    ee = 2 * g.double().abs() + 3
+    ef, eom = om * ee + 4, f * ee + 4
+    x, dy, dlast, f, om, ef, eom = (
+        a.detach().double().cpu().numpy()
+        for a in (x, dy, dlast, f, om, ef, eom))
+    c0 = np.zeros((B, D)) if state is None \
+        else state.detach().double().cpu().numpy()
+    out = {k: (np.zeros(x.shape), np.zeros(x.shape))
+           for k in ("y", "dx", "dg", "dg_plain")}
+    out.update({k: (np.zeros(c0.shape), np.zeros(c0.shape))
+                for k in ("last", "dstate")})
+
+    def put(name, at, v, e):
+        out[name][0][at], out[name][1][at] = v, e * MORE
+    relu = act == "relu"
+    for b in range(B):
+        n = T if lens is None else min(max(int(lens[b]), 0), T)
+        order = list(range(n))[::-1] if reverse else list(range(n))
+        c, M, E = c0[b], abs(c0[b]), np.zeros(D)
+        prev, side = [], []
+        for i, t in enumerate(order):
+            if states is not None and i % 64 == 0:
+                c = torch.from_numpy(c).to(states).double().numpy()
+            prev.append((c, (E + JOINS * M) * U if i else E))
+            F, a = f[b, t], om[b, t] * x[b, t]
+            c = F * c + a
+            E = F * (E + (ef[b, t] + 2) * M) + abs(a) * (eom[b, t] + 2)
+            M = F * M + abs(a)
+            bound = (E + JOINS * M) * U
+            on = c > 0 if relu else np.ones(D)
+            side.append((on, abs(c) <= bound * MORE if relu else 0 * c))
+            put("y", (b, t), c * on, bound)
+        put("last", b, c, (E + JOINS * M) * U if n else E)
+        mu, K = dlast[b], abs(dlast[b])
+        Em, Am = np.zeros(D), np.zeros(D)
+        for i in range(n - 1, -1, -1):
+            t = order[i]
+            if drop and i % drop == drop - 1:
+                mu = 0 * mu
+            (on, maybe), (p, pe) = side[i], prev[i]
+            lam, L = on * dy[b, t] + mu, abs(dy[b, t]) + K
+            El, Al = Em + L, Am + maybe * abs(dy[b, t])
+            bl, al = (El + JOINS * L) * U + Al, abs(lam)
+            F, O, rf, ro = f[b, t], om[b, t], ef[b, t], eom[b, t]
+            put("dx", (b, t), O * lam, O * (bl + al * (ro + 1) * U))
+            w = p - x[b, t]
+            we = pe + U * abs(w)
+            e = F * O * (bl * (abs(w) + we) + al * we
+                         + al * abs(w) * (rf + ro + 4) * U)
+            put("dg", (b, t), F * O * w * lam, e)
+            # off the GPU the sigmoids are differentiated one by one: 1 - f
+            # and 1 - om are off by what f and om are and a rounding, and
+            # neither cancels with the other side's
+            put("dg_plain", (b, t), F * O * w * lam, e + U * al * (
+                abs(p) * F * (rf * F + 1 + 4 * O)
+                + abs(x[b, t]) * O * (ro * O + 1 + 4 * F)))
+            mu, K = F * lam, F * L
+            Em, Am = F * (El + (rf + 1) * L), F * Al
+        put("dstate", b, mu, (Em + JOINS * K) * U + Am if n else Em)
+    return {k: tuple(torch.from_numpy(a) for a in v) for k, v in out.items()}
+
+
+def limits(want, dtype):
+    """How far a result of this type may be from the value."""
+    half = torch.finfo(dtype).eps / 2
+    v, e = want
+    return e + half * (v.abs() + e) + torch.finfo(dtype).tiny * half
+
+
+def within(name, got, want, dtype):
+    assert got.dtype == dtype and got.shape == want[0].shape, name
+    err = (got.detach().double().cpu() - want[0]).abs()
+    lim = limits(want, dtype)
+    assert bool((err <= lim).all()), \
+        f"{name}: {float((err / lim.clamp_min(1e-300)).max())} of the limit"
+
+
+SHARP_CASES = [
+    dict(B=2, T=1, D=3, dtype=torch.float32),
+    dict(B=3, T=17, D=30, dtype=torch.float16, lens="ragged"),
+    dict(B=2, T=65, D=257, dtype=torch.float32, act="relu"),
+    dict(B=4, T=130, D=130, dtype=torch.bfloat16, lens="ragged", reverse=True,
+         act="relu", layout="fused"),
+    dict(B=1, T=1000, D=70, dtype=torch.float32, reverse=True),
+    dict(B=1, T=1025, D=256, dtype=torch.bfloat16, layout="fused"),
+    dict(B=1, T=1025, D=256, dtype=torch.bfloat16, layout="fused",
+         act="relu"),
+    dict(B=7, T=700, D=40, dtype=torch.float32, lens="ragged", act="relu"),
+    dict(B=7, T=700, D=41, dtype=torch.bfloat16, lens="ragged", reverse=True),
+    dict(B=3, T=1500, D=66, dtype=torch.float16, act="relu", layout="fused",
+         state=False),
+    dict(B=1, T=4200, D=1, dtype=torch.float16),
+    dict(B=1, T=4200, D=33, dtype=torch.float32, act="relu", reverse=True),
+    # not split: many blocks
+    dict(B=40, T=150, D=330, dtype=torch.float32, act="relu", lens="ragged"),
+]
+
+
+def sharp_case(dev, B, T, D, dtype, lens=None, reverse=False, act="none",
+               state=True, layout="split"):
+    xg, st, ln, dy, dlast = make(B, T, D, dtype, dev, 21, state, lens)
+    want = sharp(xg[..., :D], xg[..., D:], st, ln, reverse, act, dy, dlast)
+    kw = dict(state=st, lens=ln, reverse=reverse, act=act)
+    leaves = [] if st is None else [st.requires_grad_()]
+    if layout == "fused":
+        leaves = [xg.requires_grad_()] + leaves
+        y, last = ops.gated_scan_xg(xg, **kw)
+    else:
+        x, g = (a.contiguous().requires_grad_()
+                for a in (xg[..., :D], xg[..., D:]))
+        leaves = [x, g] + leaves
+        y, last = ops.gated_scan(x, g, **kw)
+    grads = torch.autograd.grad((y, last), leaves, (dy, dlast))
+    if layout == "fused":
+        grads = (grads[0][..., :D], grads[0][..., D:]) + grads[1:]
+    within("y", y, want["y"], dtype)
+    within("last", last, want["last"], torch.float32)
+    within("dx", grads[0], want["dx"], dtype)
+    within("dg", grads[1], want["dg" if dev == "cuda" else "dg_plain"], dtype)
+    if st is not None:
+        within("dstate", grads[2], want["dstate"], torch.float32)
+
+
+@pytest.mark.parametrize("case", SHARP_CASES)
+def test_scan_plain_within_damped_bounds(case):
+    sharp_case("cpu", **{**case, "B": min(case["B"], 4)})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", SHARP_CASES)
+def test_scan_gpu_within_damped_bounds(case):
+    sharp_case("cuda", **case)
+
+
+@pytest.mark.parametrize("T,D", [(1000, 70), (1025, 64), (4200, 16)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16,
+                                   torch.float16])
+def test_damped_bounds_reject_mistakes(T, D, dtype):
+    """Planted in the oracle: no gate gradient, a carry lost every 64 steps or
+    every 2048, tile states kept in 16 bits."""
+    xg, st, _, dy, dlast = make(1, T, D, dtype, "cpu", 22)
+    args = (xg[..., :D], xg[..., D:], st, None, False, "none", dy, dlast)
+    right = sharp(*args)
+    out = lambda name, v, t: ((v - right[name][0]).abs()
+                              > limits(right[name], t)).double().mean()
+    assert out("dg", torch.zeros_like(right["dg"][0]), dtype) > 0.9
+    for drop, share in ((64, 64), (2048, 2048)):
+        if T > drop:
+            lost = sharp(*args, drop=drop)
+            # the step before each loss sees it at once
+            for k in ("dx", "dg"):
+                assert out(k, lost[k][0], dtype) > 0.5 / share
+    few = sharp(*args, states=torch.bfloat16)
+    if dtype == torch.float32:
+        assert out("y", few["y"][0], dtype) > 0.02
+        assert out("dg", few["dg"][0], dtype) > 0.005
+    if T % 64 == 1:     # 40 steps behind its mistake a state has lost it
+        assert out("last", few["last"][0], torch.float32) > 0.1
