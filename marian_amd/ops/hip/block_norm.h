@@ -364,10 +364,8 @@ __global__ __launch_bounds__(MAXT) void join_fwd_kernel(NormArgs a) {
   // the same number of turns for all lanes of a wave
   for (long r0 = 0, n = (a.rows + it.stride - 1) / it.stride; r0 < n; ++r0) {
     const long row = it.row + r0 * it.stride;
-    // waves that meet at barriers leave together
-    if ((PLACE == kPair ? it.row0 + r0 * it.stride : row) >= a.rows &&
-        PLACE != kPartWave)
-      break;
+    // waves that meet at barriers work on one row
+    if (PLACE != kPartWave && row >= a.rows) break;
     if (!KEEP) fetch(row);
     const bool on = !may_idle(PLACE) || row < a.rows;
     const long base = row * a.D;
@@ -669,10 +667,10 @@ struct NormPlan {
 
 #define GATES(T, VEC, EPT, PLACE, POST, PRE, MAXT, FN)                    \
   switch (pl.gate) {                                                      \
-    case kNone: FN(T, VEC, EPT, PLACE, POST, PRE, kNone, MAXT) break;     \
-    case kScaleCh: FN(T, VEC, EPT, PLACE, POST, PRE, kScaleCh, MAXT) break;   \
-    case kScaleTok: FN(T, VEC, EPT, PLACE, POST, PRE, kScaleTok, MAXT) break;  \
-    case kHighCh: FN(T, VEC, EPT, PLACE, POST, PRE, kHighCh, MAXT) break;     \
+    case kNone: FN(T, VEC, EPT, PLACE, POST, PRE, kNone, MAXT)            \
+    case kScaleCh: FN(T, VEC, EPT, PLACE, POST, PRE, kScaleCh, MAXT)      \
+    case kScaleTok: FN(T, VEC, EPT, PLACE, POST, PRE, kScaleTok, MAXT)    \
+    case kHighCh: FN(T, VEC, EPT, PLACE, POST, PRE, kHighCh, MAXT)        \
     default: FN(T, VEC, EPT, PLACE, POST, PRE, kHighTok, MAXT)            \
   }
 #define SIDES(T, VEC, EPT, PLACE, MAXT, FN)                               \
@@ -685,17 +683,32 @@ struct NormPlan {
   } else {                                                                \
     GATES(T, VEC, EPT, PLACE, false, false, MAXT, FN)                     \
   }
-#define WIDTHS(T, FN)                                                     \
+// The widths' kernels that both passes have, and those of one of them.
+#define NARROW(T, FN)                                                     \
   constexpr int V = 16 / (int)sizeof(T);                                  \
-  if (pl.ept == 1) { SIDES(T, 1, 1, kPartWave, 256, FN) }                 \
-  else if (pl.place == kPartWave) { SIDES(T, V, 8, kPartWave, 256, FN) }  \
-  else if (pl.place == kWave && pl.ept == 8) {                            \
+  if (pl.ept == 1) {                                                      \
+    SIDES(T, 1, 1, kPartWave, 256, FN)                                    \
+  } else if (pl.place == kPartWave) {                                     \
+    SIDES(T, V, 8, kPartWave, 256, FN)                                    \
+  } else if (pl.place == kWave && pl.ept == 8) {                          \
     SIDES(T, V, 8, kWave, 256, FN)                                        \
-  } else if (pl.place == kWave) { SIDES(T, V, 16, kWave, 256, FN) }       \
-  else if (pl.place == kPair) { SIDES(T, V, 8, kPair, 256, FN) }          \
-  else if (pl.ept == 8) { SIDES(T, V, 8, kBlock, 512, FN) }               \
-  else if (pl.threads <= 512) { SIDES(T, V, 16, kBlock, 512, FN) }        \
-  else { SIDES(T, V, 16, kBlock, 1024, FN) }
+  }
+#define WIDE(T, FN)                                                       \
+  if (pl.place == kBlock && pl.ept == 8) {                                \
+    SIDES(T, V, 8, kBlock, 512, FN)                                       \
+  } else if (pl.place == kBlock && pl.threads <= 512) {                   \
+    SIDES(T, V, 16, kBlock, 512, FN)                                      \
+  } else if (pl.place == kBlock) {                                        \
+    SIDES(T, V, 16, kBlock, 1024, FN)                                     \
+  }
+#define FWD_WIDTHS(T, FN)                                                 \
+  NARROW(T, FN) else if (pl.place == kWave) {                             \
+    if constexpr (sizeof(T) == 2) { SIDES(T, V, 16, kWave, 256, FN) }     \
+  } else WIDE(T, FN)
+#define BWD_WIDTHS(T, FN)                                                 \
+  NARROW(T, FN) else if (pl.place == kPair) {                             \
+    SIDES(T, V, 8, kPair, 256, FN)                                        \
+  } else WIDE(T, FN)
 
 // blocks of a kernel that a CU holds at once, asked for once per block size
 template <auto KERNEL>
@@ -713,7 +726,8 @@ int resident(int threads) {
   return n;
 }
 
-// grid == 0: nothing is launched, the blocks that a CU holds are returned
+// grid == 0: nothing is launched, the blocks that a CU holds are returned.
+// 0 is returned where there is no kernel for the plan.
 template <typename T>
 int join_fwd_launch(const NormPlan& pl, unsigned grid, hipStream_t stream) {
   const NormArgs& a = pl.a;
@@ -723,8 +737,9 @@ int join_fwd_launch(const NormPlan& pl, unsigned grid, hipStream_t stream) {
         &join_fwd_kernel<T, VEC, EPT, PLACE, POST, PRE, GATE, MAXT>;         \
     if (grid == 0) return resident<kernel>(pl.threads);                      \
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(pl.threads), 0, stream, a);  \
+    return 1;                                                                \
   }
-  WIDTHS(T, RUN)
+  FWD_WIDTHS(T, RUN)
 #undef RUN
   return 0;
 }
@@ -745,13 +760,17 @@ int join_bwd_launch(const NormPlan& pl, unsigned grid, hipStream_t stream) {
                      : resident<kernel>(pl.threads);                         \
     hipLaunchKernelGGL(is_lean ? lean : kernel, dim3(grid),                  \
                        dim3(pl.threads), 0, stream, a);                      \
+    return 1;                                                                \
   }
-  WIDTHS(T, RUN)
+  BWD_WIDTHS(T, RUN)
 #undef RUN
   return 0;
 }
 
-#undef WIDTHS
+#undef BWD_WIDTHS
+#undef FWD_WIDTHS
+#undef WIDE
+#undef NARROW
 #undef SIDES
 #undef GATES
 

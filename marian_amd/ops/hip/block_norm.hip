@@ -194,6 +194,7 @@ int dispatch(bool bwd, const torch::Tensor& x, const NormPlan& pl,
             : join_fwd_launch<float>(pl, grid, stream);
   else
     TORCH_CHECK(false, "block_norm: unsupported dtype");
+  TORCH_CHECK(n > 0, "block_norm: no kernel for this plan");
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return n;
 }

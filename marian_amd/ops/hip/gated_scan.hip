@@ -745,9 +745,12 @@ void launch(bool bwd, const torch::Tensor& x, const ScanArgs& a,
   else                                                                       \
     hipLaunchKernelGGL((scan_fwd_kernel<ET, VEC, NW, AGG>), grid,            \
                        dim3(NW * 64), 0, stream, a)
+// one wave holds all of the steps: there are no chunks
 #define RUN1(ET, VEC)                                                        \
-  if (nw == 1) { RUN2(ET, VEC, 1); }                                         \
-  else { RUN2(ET, VEC, 4); }
+  if (nw == 1) {                                                             \
+    if constexpr (AGG) TORCH_CHECK(false, "gated_scan: no such chunks");     \
+    else { RUN2(ET, VEC, 1); }                                               \
+  } else { RUN2(ET, VEC, 4); }
 #define RUN(ET)                                                              \
   if (vec_of_width(a.D) == 2) { RUN1(ET, 2) } else { RUN1(ET, 1) }
   SCAN_DTYPES(x.scalar_type(), RUN)

@@ -589,3 +589,38 @@ def oracle_with_bias(t, bias):
     zero = torch.zeros(t["x"].shape[-1], device=t["x"].device)
     return oracle({k: zero if v is None and k.endswith("bias") else v
                    for k, v in t.items()}, "rms", "scale", 1.0)
+
+
+def test_every_kernel_has_a_width():
+    """The extension holds the kernels that some width picks, and no others:
+    (vector, elements a lane, place of a row's lanes, threads at most)."""
+    import re
+    from marian_amd.ops import _load
+    path = _load.extension_path()
+    if path is None:
+        pytest.skip("the extension is not built")
+    part_wave, wave, pair, block = range(4)
+
+    def plan(D, vec, bwd):
+        if D < vec:
+            return 1, 1, part_wave, 256
+        if D <= 256:
+            return vec, 8, part_wave, 256
+        if D <= 512:
+            return vec, 8, wave, 256
+        if D <= 1024:
+            return (vec, 8, pair, 256) if bwd else \
+                (vec, 16, wave, 256) if vec == 8 else (vec, 8, block, 512)
+        if D <= 4096:
+            return vec, 8, block, 512
+        return vec, 16, block, 512 if D <= 8192 else 1024
+    with open(path, "rb") as f:
+        names = set(re.findall(
+            rb"join_(fwd|bwd)_kernelI(f|DF16b|DF16_)Li(\d+)ELi(\d+)ELi(\d+)E"
+            rb"Lb[01]ELb[01]ELi\d+ELi(\d+)E", f.read()))
+    for way in ("fwd", "bwd"):
+        for name, vec in (("f", 4), ("DF16b", 8), ("DF16_", 8)):
+            held = {tuple(map(int, n[2:])) for n in names
+                    if n[0].decode() == way and n[1].decode() == name}
+            assert held == {plan(D, vec, way == "bwd")
+                            for D in range(1, 16385)}, (way, name)

@@ -744,3 +744,19 @@ def test_damped_bounds_reject_mistakes(T, D, dtype):
         assert out("dg", few["dg"][0], dtype) > 0.005
     if T % 64 == 1:     # 40 steps behind its mistake a state has lost it
         assert out("last", few["last"][0], torch.float32) > 0.1
+
+
+def test_every_kernel_is_reached():
+    """(channels a lane, waves, chunks' maps): one wave has no chunks."""
+    import re
+    from marian_amd.ops import _load
+    path = _load.extension_path()
+    if path is None:
+        pytest.skip("the extension is not built")
+    with open(path, "rb") as f:
+        names = set(re.findall(rb"scan_(fwd|bwd)_kernelI(?:f|DF16b|DF16_)"
+                               rb"Li(\d+)ELi(\d+)ELb([01])E", f.read()))
+    held = {tuple(map(int, n[1:])) for n in names}
+    assert {n[0] for n in names} == {b"fwd", b"bwd"}
+    assert held == {(v, 4, m) for v in (1, 2) for m in (0, 1)} \
+        | {(v, 1, 0) for v in (1, 2)}
