@@ -748,8 +748,8 @@ void launch(bool bwd, const torch::Tensor& x, const ScanArgs& a,
 // one wave holds all of the steps: there are no chunks
 #define RUN1(ET, VEC)                                                        \
   if (nw == 1) {                                                             \
-    if constexpr (AGG) TORCH_CHECK(false, "gated_scan: no such chunks");     \
-    else { RUN2(ET, VEC, 1); }                                               \
+    TORCH_CHECK(!AGG, "gated_scan: no such chunks");                         \
+    if constexpr (!AGG) { RUN2(ET, VEC, 1); }                                \
   } else { RUN2(ET, VEC, 4); }
 #define RUN(ET)                                                              \
   if (vec_of_width(a.D) == 2) { RUN1(ET, 2) } else { RUN1(ET, 1) }
