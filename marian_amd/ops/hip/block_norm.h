@@ -429,10 +429,16 @@ __global__ __launch_bounds__(MAXT) void join_bwd_kernel(NormArgs a) {
   // blocks of 1024 have 128 registers a lane: parameters are read again for
   // each row and nothing is fetched ahead
   constexpr bool KEEP = MAXT <= 512;
-  // rows of 16 elements a lane leave no registers for the next row's, except
-  // where the sums are few (4096 x 6000: 75 us for 85); a highway's spill
-  constexpr bool AHEAD = KEEP && (!(PLACE == kBlock && EPT == 16) ||
-                                 (LEAN && !is_highway(GATE)));
+  // Rows of 16 elements a lane leave no registers for the next row's, except
+  // where the sums and the operands are few. rms, this kernel alone, with the
+  // fetch ahead and without: 2048 x 8192 bf16 no gate 37.6 us for 40.5 with a
+  // pre norm and 47.4 for 47.1 with both, 2048 x 6000 37.8 for 38.9, with a
+  // factor 38.9 for 39.9 (44.6 for 43.8 at 8192 and a pre norm). Gates per
+  // token gain nothing, and fp32 spills: a whole pass of 4096 x 6000 with a
+  // factor and both norms takes 303 us for 199.
+  constexpr bool FEW =
+      LEAN && sizeof(T) == 2 && (GATE == kNone || GATE == kScaleCh);
+  constexpr bool AHEAD = KEEP && (!(PLACE == kBlock && EPT == 16) || FEW);
   using Raw = RawRow<T, VEC, NC>;
   __shared__ float buf[2][32];
   // the lane groups' sums of one parameter
