@@ -298,13 +298,15 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor,
     reverse: the steps run from position lens[b]-1 down to 0.
     y: [B, T, D] in x's dtype; last: float32 [B, D], the state after the last
     step (`state` itself for a row of no steps). States are held in 32 bits.
-    Differentiable once in x, gate and state; on the GPU neither forward-mode
-    derivatives nor traces are taken.
+    Differentiable once in x, gate and state; on the GPU forward-mode
+    derivatives are refused. Traces are refused everywhere: they would hold
+    the outputs, or the number of steps.
     """
     if _on_gpu(x):
         return hip_ext(required=True).gated_scan(x, gate, state, lens,
                                                  reverse, act)
-    from ._gated_scan import check_scan, gated_scan_torch
+    from ._gated_scan import check_scan, check_untraced, gated_scan_torch
+    check_untraced("gated_scan")
     check_scan("gated_scan", x, gate, state, lens, act, 3)
     return gated_scan_torch(x, gate, state, lens, reverse, act)
 
@@ -317,7 +319,8 @@ def gated_scan_xg(xg: torch.Tensor, state: Optional[torch.Tensor] = None,
     if _on_gpu(xg):
         return hip_ext(required=True).gated_scan_xg(xg, state, lens, reverse,
                                                     act)
-    from ._gated_scan import check_scan, gated_scan_torch
+    from ._gated_scan import check_scan, check_untraced, gated_scan_torch
+    check_untraced("gated_scan_xg")
     if xg.dim() != 3 or xg.shape[-1] % 2:
         raise ValueError("gated_scan_xg: xg must be [B, T, 2D], got "
                          f"{tuple(xg.shape)}")

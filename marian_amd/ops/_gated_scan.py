@@ -41,6 +41,12 @@ def check_scan(what, x, gate, state, lens, act, dims):
                          "device")
 
 
+def check_untraced(what):
+    if torch.jit.is_tracing():
+        raise NotImplementedError(f"{what} cannot be traced: the trace would "
+                                  "hold the number of steps")
+
+
 def gated_scan_torch(x, gate, state=None, lens=None, reverse=False,
                      act="none"):
     """The recurrence step by step in (at least) 32 bits."""

@@ -708,10 +708,13 @@ ScanArgs base_args(const torch::Tensor& x, const torch::Tensor& g,
   a.ctiles = (a.D + vec_of_width(a.D) * kLC - 1) / (vec_of_width(a.D) * kLC);
   a.nt = (a.T + tile - 1) / tile;
   const long pairs = (long)a.B * a.ctiles;
-  // Blocks that walk all of the time axis are faster from about 192 of them
-  // on: the chunks' maps cost another reading of the inputs (16 x 2048 x 1024
-  // bf16, 256 blocks: 47 + 82 us, split 56 + 95). Below that, two blocks per
-  // CU: 512 or 2048 of them made no difference at 1 x 16384 x 1024.
+  // The chunks' maps cost another reading of the inputs, so the time axis is
+  // split only where blocks that walk all of it are few. Forward and backward
+  // with relu at 2048 x 1024, split and walked: bf16 8 sequences (128 blocks)
+  // 90 and 125 us, 10 104 and 125, 12 131 and 126, 16 159 and 130; fp32 8 159
+  // and 167, 10 189 and 176, 12 235 and 185; 12 x 16384 x 1024 bf16 1139 and
+  // 945. Up to two blocks per CU, in at most 32 chunks: fewer than 16 tiles of
+  // channels leave CUs without one (1 x 16384 x 64: 64 us, walked 896).
   const int nc = pairs >= 192 || pairs == 0
                      ? 1
                      : (int)std::min<long>({kMaxChunks, (long)a.nt,

@@ -62,6 +62,10 @@ class _DecoderStep(torch.nn.Module):
 def export_onnx(model, prefix: str, vocab_size: int) -> list:
     """Write <prefix>.encoder.onnx / <prefix>.decoder.onnx; returns the
     file list. Model must be a TransformerModel on CPU in eval mode."""
+    if model.opt.get("transformer-decoder-autoreg", "") == "rnn":
+        # a trace holds the number of steps that it has seen
+        raise ValueError("ONNX export does not take a recurrent decoder "
+                         "(--transformer-decoder-autoreg rnn)")
     model = model.float().cpu().eval()
     _patch_missing_onnx()
     B, Ts, Tt = 2, 5, 3

@@ -284,6 +284,21 @@ def test_gpu_calls_refuse_modes(dev):
                   s)
 
 
+def test_traces_off_the_gpu():
+    """A scan's trace would hold the number of steps; a single step's does
+    not."""
+    xg, st, _, _, _ = make(2, 3, 4, torch.float32, "cpu", 3)
+    for fn in (lambda a, s: ops.gated_scan_xg(a, s),
+               lambda a, s: ops.gated_scan(a[..., :4], a[..., 4:], s)):
+        with pytest.raises(NotImplementedError, match="traced"):
+            torch.jit.trace(fn, (xg, st), check_trace=False)
+    step = lambda a, s: ops.gated_step(a[:, :4], a[:, 4:], s, act="relu")
+    traced = torch.jit.trace(step, (xg[:, 0], st), check_trace=False)
+    more = torch.randn(5, 8), torch.randn(5, 4)
+    for a, b in zip(traced(*more), step(*more)):
+        assert torch.equal(a, b)
+
+
 def test_forward_mode_off_the_gpu():
     """There the tangent comes out: against differences."""
     import torch.autograd.forward_ad as fwd

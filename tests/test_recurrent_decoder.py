@@ -236,6 +236,20 @@ def test_projection_with_int8_weights():
     assert not torch.equal(got, want)
 
 
+def test_export(tmp_path):
+    """A recurrent decoder is refused before a file is written; the other
+    decoders export with the fused pre/postprocess ops."""
+    from marian_amd.translator.onnx_export import export_onnx
+    with pytest.raises(ValueError, match="recurrent"):
+        export_onnx(create_model(options("n", "da")), str(tmp_path / "m"), 37)
+    assert not list(tmp_path.iterdir())
+    for pre, post in (("r", "drga"), ("n", "dh"), ("", "dhn")):
+        m = create_model(options(pre, post, 0.5, **{
+            "transformer-decoder-autoreg": "self-attention"}))
+        for f in export_onnx(m, str(tmp_path / "m"), 37):
+            assert (tmp_path / f).stat().st_size > 0
+
+
 # ------------------------------------------------------------------ on the GPU
 
 @pytest.mark.gpu
