@@ -353,9 +353,8 @@ def gated_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor,
             raise ValueError("gated_step: inplace has no gradient")
         if not state.is_contiguous():
             raise ValueError("gated_step: inplace needs a dense state")
-        own = state.untyped_storage().data_ptr()
-        if own in (x.untyped_storage().data_ptr(),
-                   gate.untyped_storage().data_ptr()):
+        own = state.untyped_storage()._cdata    # empty ones share address 0
+        if own in (x.untyped_storage()._cdata, gate.untyped_storage()._cdata):
             raise ValueError("gated_step: inplace needs a state of its own "
                              "memory")
     y, new = gated_scan_torch(x[:, None], gate[:, None], state, act=act)

@@ -319,6 +319,36 @@ def test_outputs_may_be_changed_in_place(dev, lead, pre):
         assert torch.equal(p, q)
 
 
+@pytest.mark.parametrize("dev", ["cpu", pytest.param(
+    "cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("name", ["x", "res", "gate", "pre_scale"])
+def test_broadcast_inputs(dev, name):
+    """An expanded input, and the sum that its gradient is."""
+    t = make(5, 24, torch.float32, dev, gate="scale", per_token=True)
+    one = t[name][:1].clone().requires_grad_()
+    shape = t[name].shape
+    res = []
+    for full in (one.expand(shape), one.expand(shape).contiguous()):
+        o = call({**t, name: full}, "layer", "scale", 0.5)
+        d = [(a, b) for a, b in zip(o, (t["dsum"], t["dh"]))
+             if a.requires_grad]
+        res.append(o + torch.autograd.grad([a for a, _ in d], one,
+                                           [b for _, b in d]))
+    assert res[0][2].shape == one.shape
+    assert all(torch.equal(p, q) for p, q in zip(*res))
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param(
+    "cuda", marks=pytest.mark.gpu)])
+def test_inference_mode(dev):
+    t = make(6, 24, torch.bfloat16, dev, gate="highway")
+    want = call(t, "layer", "highway", 0.5)
+    with torch.inference_mode():
+        got = call(t, "layer", "highway", 0.5)
+    assert all(o.is_inference() for o in got)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
 # ------------------------------------------------------------------ on the GPU
 
 GPU_CASES = [
@@ -452,6 +482,29 @@ def test_gpu_repeats_bit_for_bit():
         assert torch.equal(first[0], again[0])
         assert torch.equal(first[1], again[1])
         assert all(torch.equal(first[2][k], again[2][k]) for k in first[2])
+
+
+@pytest.mark.gpu
+def test_gpu_two_streams_at_once():
+    """Calls that overlap on two streams share nothing."""
+    jobs = []
+    for seed, D in ((1, 300), (2, 1024)):
+        t = make(3000, D, torch.bfloat16, "cuda", gate="scale", seed=seed)
+
+        def once(t=t):
+            s, h, g = run(t, "layer", "scale", 1.0)
+            return [s, h] + list(g.values())
+        jobs.append((once, torch.cuda.Stream(), once()))
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for (once, side, _), outs in zip(jobs, got):
+            with torch.cuda.stream(side):
+                outs.append(once())
+    torch.cuda.synchronize()
+    for (_, _, want), outs in zip(jobs, got):
+        for o in outs:
+            assert all(torch.equal(p, q) for p, q in zip(o, want))
 
 
 @pytest.mark.gpu

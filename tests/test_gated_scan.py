@@ -327,6 +327,74 @@ def test_last_state_has_memory_of_its_own(dev, T, lens):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+def test_empty_batches(dev):
+    for B, T in ((0, 3), (0, 100), (2, 0), (0, 0)):
+        xg = torch.zeros(B, T, 8, device=dev, requires_grad=True)
+        st = torch.ones(B, 4, device=dev, requires_grad=True)
+        y, last = ops.gated_scan_xg(xg, st)
+        assert y.shape == (B, T, 4) and torch.equal(last, st)
+        a, b = torch.autograd.grad((y, last), (xg, st), (
+            torch.ones_like(y), torch.ones_like(last)))
+        assert a.shape == xg.shape and torch.equal(b, torch.ones_like(st))
+    x, st = torch.zeros(0, 4, device=dev), torch.zeros(0, 4, device=dev)
+    for inplace in (False, True):
+        y, new = ops.gated_step(x, x.clone(), st, inplace=inplace)
+        assert y.shape == new.shape == (0, 4)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("T", [5, 70])
+def test_lengths_outside_the_axis(dev, T):
+    """Lengths are clamped to 0..T."""
+    xg, st, _, dy, dl = make(4, T, 6, torch.float32, dev, 12)
+    xg.requires_grad_(), st.requires_grad_()
+    res = []
+    for lens in ([-3, T + 9, 2 ** 31 - 1, -2 ** 31], [0, T, T, 0]):
+        ln = torch.tensor(lens, dtype=torch.int32, device=dev)
+        for rev in (False, True):
+            o = ops.gated_scan_xg(xg, st, ln, rev)
+            res.append(o + torch.autograd.grad(o, (xg, st), (dy, dl)))
+    for a, b in ((0, 2), (1, 3)):
+        assert all(torch.equal(p, q) for p, q in zip(res[a], res[b]))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dims", [(0,), (1,), (0, 1), (2,), (0, 1, 2)])
+def test_broadcast_inputs(dev, dims):
+    """Expanded inputs, and the sums that their gradients are."""
+    xg, st, _, dy, dl = make(3, 70, 6, torch.float64 if dev == "cpu" else
+                             torch.float32, dev, 13)
+    x, g = (a.clone() for a in (xg[..., :6], xg[..., 6:]))
+    for d in dims:
+        x, g = x.narrow(d, 0, 1), g.narrow(d, 0, 1)
+    x, g = x.clone().requires_grad_(), g.clone().requires_grad_()
+    res = []
+    for full in (lambda a: a.expand(3, 70, 6),
+                 lambda a: a.expand(3, 70, 6).contiguous()):
+        o = ops.gated_scan(full(x), full(g), st)
+        res.append(o + torch.autograd.grad(o, (x, g), (dy, dl)))
+    assert res[0][2].shape == x.shape
+    # off the GPU torch sums the two layouts in another order: up to 1260 terms
+    # in 64 bits are within 1260 x 2^-53 of the sum of their sizes, below 2^14
+    lim = 0 if dev == "cuda" else 1260 * 2.0 ** -53 * 2 ** 14
+    for p, q in zip(*res):
+        assert float((p - q).abs().max()) <= lim
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_inference_mode(dev):
+    xg, st, ln, _, _ = make(3, 20, 6, torch.bfloat16, dev, 14, True, "ragged")
+    want = ops.gated_scan_xg(xg, st, ln) + ops.gated_step(
+        xg[:, 0, :6], xg[:, 0, 6:], st)
+    with torch.inference_mode():
+        own = st.clone()
+        got = ops.gated_scan_xg(xg, st, ln) + ops.gated_step(
+            xg[:, 0, :6], xg[:, 0, 6:], own, inplace=True)
+    assert got[3] is own and all(t.is_inference() for t in got)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_outputs_may_be_changed_in_place(dev):
     xg, st, _, _, _ = make(2, 5, 6, torch.float32, dev, 3)
     xg.requires_grad_(), st.requires_grad_()
@@ -510,6 +578,31 @@ def test_step_gpu_captured():
         torch.cuda.synchronize()
         assert torch.equal(out, ye) and torch.equal(state, eager)
     close(state, last.double().cpu(), 6 * 80 * U * 4, torch.float32)
+
+
+@pytest.mark.gpu
+def test_gpu_two_streams_at_once():
+    """Calls that overlap on two streams share nothing."""
+    jobs = []
+    for seed in (1, 2):
+        xg, st, ln, dy, dl = make(2, 3000, 96, torch.bfloat16, "cuda", seed,
+                                  True, "ragged")
+        xg.requires_grad_(), st.requires_grad_()
+
+        def once(a=xg, s=st, n=ln, d=(dy, dl)):
+            o = ops.gated_scan_xg(a, s, n)
+            return o + torch.autograd.grad(o, (a, s), d)
+        jobs.append((once, torch.cuda.Stream(), once()))
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for (once, side, _), outs in zip(jobs, got):
+            with torch.cuda.stream(side):
+                outs.append(once())
+    torch.cuda.synchronize()
+    for (_, _, want), outs in zip(jobs, got):
+        for o in outs:
+            assert all(torch.equal(p, q) for p, q in zip(o, want))
 
 
 @pytest.mark.gpu
