@@ -57,10 +57,14 @@ __global__ __launch_bounds__(1024) void param_sum_kernel(SumArgs a) {
   for (int p = 0; p < NP; ++p) buf[p][grp][lane] = t[p];
   __syncthreads();
   if (grp < NP) {  // group p adds up the p-th sum
-    float v = 0.f;
-#pragma unroll 16
-    for (int i = 0; i < 64; ++i) v += buf[grp][i][lane];
-    total[grp][lane] = v;
+    float v[16] = {};  // 16 runs of 4, then pairs: fewer roundings a term
+#pragma unroll
+    for (int i = 0; i < 64; ++i) v[i % 16] += buf[grp][i][lane];
+#pragma unroll
+    for (int k = 8; k > 0; k /= 2)
+#pragma unroll
+      for (int i = 0; i < k; ++i) v[i] += v[i + k];
+    total[grp][lane] = v[0];
   }
   __syncthreads();
   if (grp != 0 || c >= a.D) return;

@@ -485,6 +485,27 @@ def test_gpu_repeats_bit_for_bit():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("R,D", [(1000, 700), (1000, 200), (1500, 1024),
+                                 (2000, 4200)])
+def test_gpu_sums_over_rows_in_pairs(R, D):
+    """dpre_bias is the sum of dh. A rounding of a partial sum v is at most
+    u v and spreads evenly, u v / sqrt(3) in the root mean square. For terms of
+    one sign partial sums grow in proportion: 64 lane groups' sums in 16 runs
+    of 4 and then in pairs have squares of 0.12 + 1.88 of the whole sum's, what
+    comes before (a block's rows, 4 to 16 blocks a group) below 0.25, the last
+    rounding 1: u S sqrt(3.25 / 3). One run of 64 has 21 in place of 2."""
+    gen = torch.Generator().manual_seed(8)
+    x = torch.randn(R, D, generator=gen).cuda()
+    dh = (torch.rand(R, D, generator=gen) + 0.5).cuda()
+    w, b = torch.ones(D).cuda(), torch.zeros(D).cuda().requires_grad_()
+    _, h = ops.block_norm(x, None, pre_scale=w, pre_bias=b)
+    got, = torch.autograd.grad(h, b, dh)
+    want = dh.double().sum(0)
+    rms = ((got.double() - want) / want).square().mean().sqrt()
+    assert float(rms) <= U * (3.25 / 3) ** 0.5
+
+
+@pytest.mark.gpu
 def test_gpu_two_streams_at_once():
     """Calls that overlap on two streams share nothing."""
     jobs = []
