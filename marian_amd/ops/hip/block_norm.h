@@ -26,17 +26,25 @@
 // its rows and adds up their parameter gradients in registers; the blocks'
 // partial rows are summed by a second kernel in a fixed order (no atomics).
 //
-// What bounds it: bytes. 65536 x 1024 bf16 with a channel gate: forward 4
-// tensors in 107 us (5.0 TB/s; a copy of 2 GB runs at 4.9), backward 6 in 173
-// with the parameter sums (4.7). On the way there: parameters and the next
-// row kept in registers and rows walked by as many blocks as the GPU holds at
-// once (250 -> 107 and 393 -> 190 us), two rows a block in the backward pass
-// (-> 173). Rows of 4097 columns on have 16 elements a lane and no registers
-// for the next row in the backward pass, unless the norms are rms without
-// biases, whose kernel has 32 sums fewer to hold; that one is as fast at 2048 x
-// 8192 (bf16 with a gate, whole pass: 78 us) and 178 us for 188 at 8192 x 8192,
-// 77 for 95 at 4096 x 6000. From 8193 columns on the backward pass spills:
-// 342 us at 2048 x 16384, 227 for rms without biases.
+// What bounds it: bytes. 65536 x 1024 bf16 with two layer norms and a channel's
+// factor: forward 4 tensors, backward 6, 284 us for both, 4.7 TB/s where a copy
+// of 2 GB runs at 4.9 (kernels in a profile, at the median: 110, and 197 + 13
+// for the parameter sums); a factor per token 355 us (4.9), a highway per token
+// 374 (4.7). What brought it there: parameters and the next row kept in
+// registers, rows walked by as many blocks as the GPU holds at once (forward
+// 250 -> 107, backward 393 -> 190) and two rows a block in the backward pass
+// (-> 173, then with four sums). float32 parameters beside 16-bit rows are read
+// again for every row: 332 us for 284.
+// Rows of 4097 columns on have 16 elements a lane, and their backward kernels
+// spill where sums and operands are many, by the compiler's report: up to 8192
+// columns only with both norms (bf16: 4 registers with a factor or a factor per
+// token, 46 and 75 with highways; fp32: 6 without a gate, 72 - 155 with one)
+// and, in fp32, 8 for a highway with one norm; rms norms without biases, whose
+// kernel has 32 sums fewer to hold, in highways alone (10 - 20). From 8193
+// columns on lanes have 128 registers and nearly all forms with a pre norm or a
+// gate spill (bf16 12 - 213, fp32 8 - 218). Kernels, bf16, layer norms and rms:
+// 2048 x 8192 61 and 48 us (75 and 48 with a factor), 2048 x 16384 with a
+// factor 362 and 221.
 //
 // The kernels are instantiated per element type, a source file each.
 #pragma once

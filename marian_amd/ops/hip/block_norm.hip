@@ -176,7 +176,8 @@ NormPlan make_plan(const torch::Tensor& x,
   while (a.tpr * pl.ept < a.D) a.tpr *= 2;
   if (pl.place == kWave) a.tpr = WAVE;
   // Two rows a block where the backward pass takes two waves each: half the
-  // partial sums to write and to add up (65536 x 1024 bf16: 173 us for 192).
+  // partial sums to write and to add up (65536 x 1024 bf16
+  // with four sums: 173 us for 192).
   if (bwd && pl.place == kBlock && a.tpr == 128) pl.place = kPair;
   pl.threads = pl.place == kBlock ? a.tpr : 256;
   pl.rpb = pl.threads / a.tpr;

@@ -16,16 +16,18 @@
 // starting at the 32-bit states that the forward pass kept at each tile's
 // start: no full-size state tensor is written or read.
 //
-// What bounds it: bytes where rows are many - forward 3 tensors, backward 5,
-// 81 and 140 us at 1024 x 64 x 1024 bf16, 4.9 and 4.8 TB/s where a copy of
-// 2 GB runs at 4.9 - and the vector units, at 31 operations per element (a
-// third of them the sigmoid), where rows are few: then the time axis is split
-// over blocks and a first pass makes the chunks' maps (1 x 16384 x 1024 bf16:
-// 15 + 21 us forward, 16 + 32 us backward; walked by 4 blocks of 256 channels
-// it took 2700). Layout, measured at 1024 x 64 x 1024 backward: 32 lanes of 2
-// channels by 2 groups of 8 steps, joined by permlane32_swap, 140 us; 16 lanes
-// of 4 channels joined by shuffles 176; 64 lanes of 2 channels with 16 steps
-// 214. Addresses as 64-bit pointers per row, 197 registers for 163, 145.
+// What bounds it: bytes where rows are many - forward 3 tensors, backward 5:
+// 1024 x 64 x 1024 bf16 takes 222 us for both, 4.8 TB/s where a copy of 2 GB
+// runs at 4.9 (kernels in a profile, where they do not follow each other, 87 +
+// 158 at the median), with relu too - and the vector units, at 31 operations
+// per element (a third of them the sigmoid), where rows are few: then the time
+// axis is split over blocks and a first pass makes the chunks' maps (1 x 16384
+// x 1024 bf16: 15 + 21 us forward, 16 + 31 us backward, with relu, whose map
+// needs the states, 23 + 31; walked by 4 blocks of 256 channels it took 2700).
+// Layout, measured at 1024 x 64 x 1024 backward, each at its best: 32 lanes of
+// 2 channels by 2 groups of 8 steps, joined by permlane32_swap, 140 us; 16
+// lanes of 4 channels joined by shuffles 176; 64 lanes of 2 channels with 16
+// steps 214. Addresses as 64-bit pointers per row, 197 registers for 163, 145.
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 
@@ -599,7 +601,7 @@ __global__ __launch_bounds__(NW * 64) void scan_bwd_kernel(ScanArgs a) {
 }
 
 // One token for each row: the recurrence at T = 1, on a pool of states. Bound
-// by bytes (4096 x 1024 bf16: 10.3 us, 5.7 TB/s) or by the launch (4 rows: 2).
+// by bytes (4096 x 1024 bf16: 10.6 us, 5.6 TB/s) or by the launch (4 rows: 2).
 // Here the last vector of a row goes element by element: in place, a state
 // must be read and written by one thread only.
 template <typename T, int VEC>
