@@ -64,6 +64,7 @@ class _Highway(torch.autograd.Function):
     """(1 - k) r + k u, k = sigmoid(g), whose gate's gradient is made of u - r:
     the sums of u ds and of r ds, which differentiating the formula gives,
     cancel where u and r have a common mean."""
+    generate_vmap_rule = True
 
     @staticmethod
     def forward(u, r, g):

@@ -267,7 +267,7 @@ def test_gpu_call_refuses_modes(dev):
 @pytest.mark.parametrize("gate", ["scale", "highway"])
 @pytest.mark.parametrize("per_token", [True, False])
 def test_plain_other_derivatives(gate, per_token):
-    """Off the GPU: forward mode, second derivatives, traces."""
+    """Off the GPU: forward mode, second derivatives, batches, traces."""
     t = make(3, 6, torch.float64, "cpu", gate=gate, per_token=per_token,
              seed=2)
     keys = [k for k in LEAVES if t[k] is not None]
@@ -278,6 +278,16 @@ def test_plain_other_derivatives(gate, per_token):
     assert torch.autograd.gradcheck(fn, leaves, check_forward_ad=True)
     assert torch.autograd.gradgradcheck(fn, leaves)
     plain = [t[k] for k in keys]
+    at = [keys.index("x"), keys.index("res")]
+    rows = lambda x, r: fn(*[x if i == at[0] else r if i == at[1] else v
+                             for i, v in enumerate(plain)])[1]
+    x, r = (torch.stack([plain[i], 3 * plain[i]]) for i in at)
+    many = torch.func.vmap(rows)(x, r)
+    jac = torch.func.vmap(torch.func.jacrev(rows))(x, r)
+    for i in range(2):
+        assert torch.allclose(many[i], rows(x[i], r[i]), rtol=1e-12)
+        assert torch.allclose(jac[i], torch.func.jacfwd(rows)(x[i], r[i]),
+                              rtol=1e-9, atol=1e-12)
     traced = torch.jit.trace(fn, plain, check_trace=False)
     other = [2 * v for v in plain]
     for a, b in zip(traced(*other), fn(*other)):
@@ -444,6 +454,23 @@ def test_gpu_partial_gradients():
         r = {n: None if v is None else v.detach() for n, v in t.items()}
         r[k] = r[k].clone().requires_grad_()
         g, = torch.autograd.grad(call(r, "layer", "highway", 1.0), r[k],
+                                 (t["dsum"], t["dh"]))
+        assert torch.equal(g, full[k]), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate", ["scale", "highway"])
+@pytest.mark.parametrize("norm,post", [("layer", True), ("rms", True),
+                                       ("layer", False)])
+@pytest.mark.parametrize("D", [3, 100, 300, 1000, 2000, 4200, 8300])
+def test_gpu_each_gradient_alone(D, norm, post, gate):
+    """A parameter's sums do not depend on which others are asked for."""
+    t = make(20, D, torch.float32, "cuda", norm=norm, gate=gate, post=post)
+    full = run(t, norm, gate, 0.5)[2]
+    for k in full:
+        r = {n: None if v is None else v.detach() for n, v in t.items()}
+        r[k] = r[k].clone().requires_grad_()
+        g, = torch.autograd.grad(call(r, norm, gate, 0.5), r[k],
                                  (t["dsum"], t["dh"]))
         assert torch.equal(g, full[k]), k
 
